@@ -582,16 +582,19 @@ __global__ __launch_bounds__(DO_WAVES * 64) void decode_out_kernel(const DecodeA
     // Leave this range's sums and count the arrival; the last range of the column block to arrive adds all of them in range
     // order.  Sums and counter are written and read with device-scope atomic accesses only: such a store is written
     // through to the memory side (the ranges ran on other CUs, maybe other XCDs, whose L2 caches do not snoop each other),
-    // such a load is not served from a stale line, and the barrier ahead of the counter update has waited for every
-    // thread's stores to be acknowledged.  No release / acquire fences: a fence in every wave (an L2 write-back and
-    // invalidation each) made this kernel four times slower, and even the one pair hung on the counter update cost 2.8 us
-    // of the kernel's 15.
+    // and such a load is not served from a stale line.  Every wave waits for its own stores to be acknowledged before the
+    // barrier ahead of the counter update; the wait is written out because a workgroup barrier alone orders LDS traffic
+    // only (its release is at workgroup scope, where stores of one CU are ordered by its own cache and need no wait): without
+    // it the counter could reach the memory side first, and the last range to arrive add up another range's old sums.
+    // No release / acquire fences: a fence in every wave (an L2 write-back and invalidation each) made this kernel four
+    // times slower, and even the one pair hung on the counter update cost 2.8 us of the kernel's 15.
     float* mine = A.partial + ((int64_t)cb * Q + q) * (DC_MAX_TOKENS * DO_COLS);
     if (t < 128) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         __hip_atomic_store(mine + t * 4 + r, o[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (t == 0) {
       const int arrived = __hip_atomic_fetch_add(A.tickets + cb, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
