@@ -96,6 +96,32 @@ int check_packed(const d2dmoe_shape& sh, const void* packed, const d2dmoe_packed
   return D2DMOE_OK;
 }
 
+inline bool aligned_elem(const void* p, int dtype) { return (((uintptr_t)p) & (elem_size(dtype) - 1)) == 0; }
+
+int check_norm_shape(const d2dmoe_norm_shape* sh) {
+  if (sh == nullptr) return D2DMOE_E_NULL;
+  if (!dtype_ok(sh->dtype) || (sh->param_dtype != sh->dtype && sh->param_dtype != D2DMOE_F32)) return D2DMOE_E_DTYPE;
+  if (sh->n_rows < 0 || sh->width <= 0 || sh->width > (1 << 24) || sh->n_rows > ((int64_t)1 << 62) / sh->width) return D2DMOE_E_SHAPE;
+  if (!(sh->eps >= 0.f && sh->eps < __builtin_inff())) return D2DMOE_E_VALUE;
+  return D2DMOE_OK;
+}
+
+// `choice`: the fields that the choice of experts goes by are read too
+int check_route_shape(const d2dmoe_route_shape* sh, bool choice) {
+  if (sh == nullptr) return D2DMOE_E_NULL;
+  if (!dtype_ok(sh->dtype)) return D2DMOE_E_DTYPE;
+  if (sh->n_tokens < 0 || sh->n_tokens > ((int64_t)1 << 48) || sh->n_experts <= 0 || sh->n_experts > 1024) return D2DMOE_E_SHAPE;
+  if (sh->k <= 0 || sh->k > sh->n_experts) return D2DMOE_E_SHAPE;
+  if (sh->scoring != D2DMOE_SCORE_SOFTMAX && sh->scoring != D2DMOE_SCORE_SIGMOID) return D2DMOE_E_VALUE;
+  if ((sh->renormalise != 0 && sh->renormalise != 1) || !(__builtin_fabsf(sh->scale) < __builtin_inff())) return D2DMOE_E_VALUE;
+  if (!choice) return D2DMOE_OK;
+  if (sh->n_groups <= 0 || sh->n_experts % sh->n_groups != 0 || sh->kept_groups <= 0 || sh->kept_groups > sh->n_groups)
+    return D2DMOE_E_SHAPE;
+  if (sh->k > sh->kept_groups * (sh->n_experts / sh->n_groups)) return D2DMOE_E_SHAPE;
+  if (sh->n_groups > 1 && sh->group_score != D2DMOE_GROUP_MAX && sh->group_score != D2DMOE_GROUP_TOP2) return D2DMOE_E_VALUE;
+  return D2DMOE_OK;
+}
+
 struct ForwardWorkspace {
   size_t hidden_off, norms_off, perm_off, total;
 };
@@ -141,6 +167,7 @@ const char* d2dmoe_status_string(int status) {
     case D2DMOE_E_ALIGN: return "tensor pointer not aligned to 16 bytes";
     case D2DMOE_E_STATIC_LIMIT: return "shape needs more workspace than the static array of d2dmoe_forward_static holds";
     case D2DMOE_E_PACKED: return "packed buffer without its descriptor, or packed for another layer or layout version";
+    case D2DMOE_E_VALUE: return "scalar argument outside its range";
     default: break;
   }
   if (status > 0) return hipGetErrorString((hipError_t)status);
@@ -556,6 +583,68 @@ int d2dmoe_expert_output_norms(const d2dmoe_shape* shape, const void* x, const v
   if (!mfma_norms_supported(*shape)) return D2DMOE_E_UNSUPPORTED;
   if (!aligned16(x) || !aligned16(packed)) return D2DMOE_E_ALIGN;
   return (int)launch_mfma_norms(*shape, x, packed, norms, (hipStream_t)stream);
+}
+
+int d2dmoe_layer_norm(const d2dmoe_norm_shape* shape, const void* x, const void* residual, const void* weight, const void* bias,
+                      void* sum, void* out, float* mean, float* rstd, void* stream) {
+  const int st = check_norm_shape(shape);
+  if (st != D2DMOE_OK) return st;
+  if (shape->n_rows == 0) return D2DMOE_OK;
+  if (!x || !out) return D2DMOE_E_NULL;
+  const int t = shape->dtype, p = shape->param_dtype;
+  if (!aligned_elem(x, t) || !aligned_elem(residual, t) || !aligned_elem(sum, t) || !aligned_elem(out, t) || !aligned_elem(weight, p) ||
+      !aligned_elem(bias, p) || !aligned_elem(mean, D2DMOE_F32) || !aligned_elem(rstd, D2DMOE_F32))
+    return D2DMOE_E_ALIGN;
+  return (int)launch_layer_norm(*shape, x, residual, weight, bias, sum, out, mean, rstd, (hipStream_t)stream);
+}
+
+size_t d2dmoe_layer_norm_workspace_bytes(const d2dmoe_norm_shape* shape) {
+  if (check_norm_shape(shape) != D2DMOE_OK) return 0;
+  return align_up(layer_norm_workspace_bytes(*shape));
+}
+
+int d2dmoe_layer_norm_backward(const d2dmoe_norm_shape* shape, const void* grad_out, const void* grad_sum, const void* h,
+                               const void* weight, const float* mean, const float* rstd, void* grad, void* grad_weight,
+                               void* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_norm_shape(shape);
+  if (st != D2DMOE_OK) return st;
+  const bool columns = grad_weight || grad_bias;
+  if (shape->n_rows == 0 && !columns) return D2DMOE_OK;
+  if (shape->n_rows > 0 && (!grad_out || !h || !mean || !rstd || (!grad && !columns))) return D2DMOE_E_NULL;
+  const int t = shape->dtype, p = shape->param_dtype;
+  if (!aligned_elem(grad_out, t) || !aligned_elem(grad_sum, t) || !aligned_elem(h, t) || !aligned_elem(grad, t) ||
+      !aligned_elem(weight, p) || !aligned_elem(grad_weight, p) || !aligned_elem(grad_bias, p) || !aligned_elem(mean, D2DMOE_F32) ||
+      !aligned_elem(rstd, D2DMOE_F32))
+    return D2DMOE_E_ALIGN;
+  const size_t need = columns ? layer_norm_workspace_bytes(*shape) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || (((uintptr_t)workspace) & 255u))) return D2DMOE_E_WORKSPACE;
+  return (int)launch_layer_norm_backward(*shape, grad_out, grad_sum, h, weight, mean, rstd, grad, grad_weight, grad_bias, workspace,
+                                         (hipStream_t)stream);
+}
+
+int d2dmoe_route_topk(const d2dmoe_route_shape* shape, const void* logits, const float* choice_bias, void* routing,
+                      int32_t* indices, float* weights, int32_t* counts, void* stream) {
+  const int st = check_route_shape(shape, true);
+  if (st != D2DMOE_OK) return st;
+  if (shape->n_tokens == 0 && !counts) return D2DMOE_OK;
+  if (!routing && !indices && !weights && !counts) return D2DMOE_E_NULL;
+  if (shape->n_tokens > 0 && !logits) return D2DMOE_E_NULL;
+  if (!aligned_elem(logits, shape->dtype) || !aligned_elem(routing, shape->dtype) || !aligned_elem(choice_bias, D2DMOE_F32) ||
+      !aligned_elem(indices, D2DMOE_F32) || !aligned_elem(weights, D2DMOE_F32) || !aligned_elem(counts, D2DMOE_F32))
+    return D2DMOE_E_ALIGN;
+  return (int)launch_route_topk(*shape, logits, choice_bias, routing, indices, weights, counts, (hipStream_t)stream);
+}
+
+int d2dmoe_route_topk_backward(const d2dmoe_route_shape* shape, const void* logits, const int32_t* indices,
+                               const void* grad_routing, const float* grad_weights, void* grad_logits, void* stream) {
+  const int st = check_route_shape(shape, false);
+  if (st != D2DMOE_OK) return st;
+  if (shape->n_tokens == 0) return D2DMOE_OK;
+  if (!logits || !indices || !grad_logits || (!grad_routing && !grad_weights)) return D2DMOE_E_NULL;
+  if (!aligned_elem(logits, shape->dtype) || !aligned_elem(grad_routing, shape->dtype) || !aligned_elem(grad_logits, shape->dtype) ||
+      !aligned_elem(indices, D2DMOE_F32) || !aligned_elem(grad_weights, D2DMOE_F32))
+    return D2DMOE_E_ALIGN;
+  return (int)launch_route_topk_backward(*shape, logits, indices, grad_routing, grad_weights, grad_logits, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -122,4 +122,18 @@ size_t mfma_norms_packed_bytes(const d2dmoe_shape& sh);
 hipError_t launch_norms_pack(const d2dmoe_shape& sh, const void* w1, const void* b1, const void* w2, void* packed, hipStream_t s);
 hipError_t launch_mfma_norms(const d2dmoe_shape& sh, const void* x, const void* packed, void* norms, hipStream_t s);
 
+// ---- layer norm (kernels_layer_norm.hip) ----
+size_t layer_norm_workspace_bytes(const d2dmoe_norm_shape& sh);
+hipError_t launch_layer_norm(const d2dmoe_norm_shape& sh, const void* x, const void* residual, const void* weight, const void* bias,
+                             void* sum, void* out, float* mean, float* rstd, hipStream_t s);
+hipError_t launch_layer_norm_backward(const d2dmoe_norm_shape& sh, const void* g, const void* gs, const void* h, const void* weight,
+                                      const float* mean, const float* rstd, void* grad, void* gw, void* gb, void* workspace,
+                                      hipStream_t s);
+
+// ---- routing by scores (kernels_route.hip) ----
+hipError_t launch_route_topk(const d2dmoe_route_shape& sh, const void* logits, const float* bias, void* routing, int32_t* indices,
+                             float* weights, int32_t* counts, hipStream_t s);
+hipError_t launch_route_topk_backward(const d2dmoe_route_shape& sh, const void* logits, const int32_t* indices, const void* g_routing,
+                                      const float* g_weights, void* grad, hipStream_t s);
+
 }  // namespace d2dmoe

@@ -1,0 +1,96 @@
+"""The operators of this package that have a backward pass, as differentiable functions on ROCm tensors: layer norm (with
+the residual added ahead of it) and routing by scores.  Forward and backward are the HIP kernels behind ``ops``; what is
+saved for the backward pass is the normalised tensor with its row statistics, or the logits with the chosen indices.
+Where no gradient is asked for, nothing is saved.  Double backward is not supported."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        out, total, mean, rstd = ops.layer_norm(x, weight, bias, eps, residual, want_stats=True)
+        ctx.save_for_backward(x if total is None else total, weight, mean, rstd)
+        ctx.bias_type = None if bias is None else bias.dtype
+        ctx.set_materialize_grads(False)
+        return out, total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_sum):
+        h, weight, mean, rstd = ctx.saved_tensors
+        want_x, want_residual, want_weight, want_bias = ctx.needs_input_grad[:4]
+        if grad_out is None:      # only the residual stream was used
+            return (grad_sum if want_x else None, grad_sum if want_residual else None, None, None, None)
+        grad, gw, gb = ops.layer_norm_backward(grad_out.contiguous(), h, weight, mean, rstd,
+                                               None if grad_sum is None else grad_sum.contiguous(),
+                                               want_grad=want_x or want_residual, want_weight=want_weight, want_bias=want_bias,
+                                               param_dtype=ctx.bias_type)
+        return (grad if want_x else None, grad if want_residual else None, gw, gb, None)
+
+
+class _RouteTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, choice_bias, k, scoring, n_groups, kept_groups, group_score, renormalise, scale, want_counts):
+        routing, indices, weights, counts = ops.route_topk(logits, k, scoring, choice_bias, n_groups, kept_groups, group_score,
+                                                           renormalise, scale, want_counts)
+        ctx.save_for_backward(logits, indices)
+        ctx.how = (scoring, renormalise, scale)
+        ctx.mark_non_differentiable(*(t for t in (indices, counts) if t is not None))
+        ctx.set_materialize_grads(False)
+        return routing, indices, weights, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_routing, _indices, grad_weights, _counts):
+        logits, indices = ctx.saved_tensors
+        grad = None
+        if ctx.needs_input_grad[0] and (grad_routing is not None or grad_weights is not None):
+            grad = ops.route_topk_backward(logits, indices, *ctx.how,
+                                           grad_routing=None if grad_routing is None else grad_routing.contiguous(),
+                                           grad_weights=None if grad_weights is None else grad_weights.contiguous())
+        return (grad,) + (None,) * 9
+
+
+def _wanted(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               residual: Optional[torch.Tensor] = None):
+    """Layer norm over the last dimension of x, or of h = x + residual; returns out without a residual and (out, h) with one.
+    Leading dimensions are free; strided inputs are copied."""
+    shape = x.shape
+    if residual is not None and residual.shape != shape:
+        raise ops.abi.D2DMoEError(f'layer_norm: residual has shape {tuple(residual.shape)}, x {tuple(shape)}')
+    x2 = x.reshape(-1, shape[-1]).contiguous()
+    r2 = None if residual is None else residual.reshape(-1, shape[-1]).contiguous()
+    if _wanted(x, residual, weight, bias):
+        out, total = _LayerNorm.apply(x2, r2, weight, bias, eps)
+    else:
+        out, total, _, _ = ops.layer_norm(x2, weight, bias, eps, r2)
+    return out.view(shape) if residual is None else (out.view(shape), total.view(shape))
+
+
+def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bias: Optional[torch.Tensor] = None,
+               n_groups: int = 1, kept_groups: int = 1, group_score: str = 'top2', renormalise: bool = True, scale: float = 1.0,
+               want_counts: bool = False):
+    """Routing by scores over the last dimension of logits (see ops.route_topk); returns (routing, indices, weights, counts)
+    with the leading dimensions of logits.  routing and weights are differentiable in the logits; the choice, and with it
+    choice_bias, has no gradient."""
+    lead = logits.shape[:-1]
+    z = logits.reshape(-1, logits.size(-1)).contiguous()
+    if choice_bias is not None:
+        choice_bias = choice_bias.detach()
+    args = (k, scoring, n_groups, kept_groups, group_score, renormalise, scale, want_counts)
+    if _wanted(logits):
+        routing, indices, weights, counts = _RouteTopk.apply(z, choice_bias, *args)
+    else:
+        routing, indices, weights, counts = ops.route_topk(z, k, scoring, choice_bias, *args[2:])
+    return routing.view(logits.shape), indices.view(*lead, k), weights.view(*lead, k), counts

@@ -3,8 +3,8 @@
 The model follows the reference's GPT (architectures/gpt.py:27-262): same module tree and parameter names
 (``transformer.wte / wpe / h.{i}.ln_1 / attn.c_attn / attn.c_proj / ln_2 / mlp.c_fc / mlp.c_proj / ln_f``, tied
 ``lm_head``), same initialisation (N(0, 0.02), residual projections scaled by 1/sqrt(2 n_layer)), so a reference
-``state_dict`` loads.  Attention is PyTorch's scaled_dot_product_attention (causal); only the feed-forward layers are
-this package's business.
+``state_dict`` loads.  Attention is PyTorch's scaled_dot_product_attention (causal); the feed-forward layers are this
+package's business, and the layer norms where their ``forward_mode`` is 'hip' (``norm.set_norm_mode``).
 
 Model surgery mirrors ``replace_with_moes`` / ``split_original_parameters`` (architectures/moe/moefication.py:104-202,
 205-306) and the patched forwards (architectures/moe/moe_models.py:79-100, 194-218):
@@ -32,6 +32,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from .layer import MoELayer, MoeficationMoE
+from .norm import NormModes, add_norm
 
 
 @dataclass
@@ -46,16 +47,13 @@ class GPTConfig:
     activation: str = 'gelu'
 
 
-class LayerNorm(nn.Module):
-    """LayerNorm with an optional bias (architectures/gpt.py:27-36)."""
+class LayerNorm(NormModes, nn.Module):
+    """LayerNorm with an optional bias (architectures/gpt.py:27-36); forward_mode 'hip' runs the HIP kernels (norm.py)."""
 
     def __init__(self, ndim, bias):
         super().__init__()
         self.weight = nn.Parameter(torch.ones(ndim))
         self.bias = nn.Parameter(torch.zeros(ndim)) if bias else None
-
-    def forward(self, x):
-        return F.layer_norm(x, self.weight.shape, self.weight, self.bias, 1e-5)
 
 
 class CausalSelfAttention(nn.Module):
@@ -107,8 +105,8 @@ class Block(nn.Module):
         self.mlp = MLP(config)
 
     def forward(self, x):
-        x = x + self.attn(self.ln_1(x))
-        return x + self.mlp(self.ln_2(x))
+        ln2, x = add_norm(self.ln_2, self.attn(self.ln_1(x)), x)
+        return x + self.mlp(ln2)
 
 
 class GPT(nn.Module):
@@ -157,8 +155,7 @@ def moe_gpt_block_forward(self, input: torch.Tensor):
     that synchronises the host)."""
     torch._assert(input.dim() == 3, f'Expected (batch_size, seq_length, hidden_dim) got {input.shape}')
     gating_data = {}
-    h = input + self.attn(self.ln_1(input))
-    ln2 = self.ln_2(h)
+    ln2, h = add_norm(self.ln_2, self.attn(self.ln_1(input)), input)
     if isinstance(self.mlp, MoELayer):
         mlp_out, ffn_gating_data = self.mlp(ln2)
         mlp_out = self.mlp.dropout(mlp_out)

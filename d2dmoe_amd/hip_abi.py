@@ -17,11 +17,14 @@ LIB_PATH = os.environ.get('D2DMOE_LIB') or os.path.join(os.path.dirname(os.path.
 F32, BF16, F16 = 0, 1, 2
 E_STATIC_LIMIT = -8
 E_PACKED = -9
+E_VALUE = -10
 PACKED_MAGIC = 0x4b50324d
 STATIC_WORKSPACE_BYTES = 256 << 20
 ACT = {'relu': 0, 'gelu': 1, 'tanh': 2, 'leaky_relu': 3, 'gelu_tanh': 4, 'silu': 5, 'identity': 6, 'abs': 7}
 PATH = {'auto': 0, 'generic': 1, 'mfma_dense': 2, 'mfma_sparse': 3, 'mfma_decode': 4, 'mfma_gemm': 5,
         'mfma_mid': 6}
+SCORING = {'softmax': 0, 'sigmoid': 1}
+GROUP_SCORE = {'max': 0, 'top2': 1}
 
 # every extern "C" symbol the header declares
 EXPORTS = (
@@ -30,6 +33,8 @@ EXPORTS = (
     'd2dmoe_build_permutation', 'd2dmoe_experts', 'd2dmoe_packed_bytes', 'd2dmoe_pack_weights', 'd2dmoe_forward',
     'd2dmoe_norms_packed_bytes', 'd2dmoe_pack_norms', 'd2dmoe_expert_output_norms', 'd2dmoe_forward_static',
     'd2dmoe_packed_desc_from_header', 'd2dmoe_packed_describe',
+    'd2dmoe_layer_norm', 'd2dmoe_layer_norm_workspace_bytes', 'd2dmoe_layer_norm_backward', 'd2dmoe_route_topk',
+    'd2dmoe_route_topk_backward',
 )
 
 
@@ -48,6 +53,19 @@ class PackedDesc(Structure):
         ('magic', c_uint32), ('layout_version', c_uint32), ('dtype', c_int32), ('d_model', c_int32), ('n_experts', c_int32),
         ('expert_dim', c_int32), ('gated', c_int32), ('router_width', c_int32), ('sections', c_uint32),
         ('reserved0', c_uint32), ('bytes', c_uint64), ('reserved1', c_uint64 * 2),
+    ]
+
+
+class NormShape(Structure):
+    """struct d2dmoe_norm_shape"""
+    _fields_ = [('n_rows', c_int64), ('width', c_int32), ('dtype', c_int32), ('param_dtype', c_int32), ('eps', c_float)]
+
+
+class RouteShape(Structure):
+    """struct d2dmoe_route_shape"""
+    _fields_ = [
+        ('n_tokens', c_int64), ('n_experts', c_int32), ('k', c_int32), ('dtype', c_int32), ('scoring', c_int32),
+        ('n_groups', c_int32), ('kept_groups', c_int32), ('group_score', c_int32), ('renormalise', c_int32), ('scale', c_float),
     ]
 
 
@@ -104,6 +122,18 @@ def load() -> ctypes.CDLL:
     lib.d2dmoe_packed_describe.argtypes = [SH, PD]
     lib.d2dmoe_packed_desc_from_header.restype = ctypes.c_int
     lib.d2dmoe_packed_desc_from_header.argtypes = [P, PD]
+    NS = POINTER(NormShape)
+    RS = POINTER(RouteShape)
+    lib.d2dmoe_layer_norm.restype = ctypes.c_int
+    lib.d2dmoe_layer_norm.argtypes = [NS, P, P, P, P, P, P, P, P, P]
+    lib.d2dmoe_layer_norm_workspace_bytes.restype = SZ
+    lib.d2dmoe_layer_norm_workspace_bytes.argtypes = [NS]
+    lib.d2dmoe_layer_norm_backward.restype = ctypes.c_int
+    lib.d2dmoe_layer_norm_backward.argtypes = [NS, P, P, P, P, P, P, P, P, P, P, SZ, P]
+    lib.d2dmoe_route_topk.restype = ctypes.c_int
+    lib.d2dmoe_route_topk.argtypes = [RS, P, P, P, P, P, P, P]
+    lib.d2dmoe_route_topk_backward.restype = ctypes.c_int
+    lib.d2dmoe_route_topk_backward.argtypes = [RS, P, P, P, P, P, P]
     _lib = lib
     return lib
 

@@ -3,7 +3,8 @@
 
 ``MoeficationMoE.forward(x[B,T,D]) -> (out[B,T,D], {name: (routing_tensor[B,T,E],)})``; the attributes
 ``forward_mode`` ('all' | 'topk' | 'dynk' | 'dynk_max'), ``tau``, ``k``, ``router``, ``experts``, ``last_bias``,
-``add_residual_connection`` keep their meaning.  ``tau`` keeps the reference's convention: an expert is kept when
+``add_residual_connection`` keep their meaning; 'softmax_topk' and 'sigmoid_topk' are this package's own (see
+``MoeficationMoE``).  ``tau`` keeps the reference's convention: an expert is kept when
 ``norm >= max_norm * (1.0 - tau)``.
 
 When ``forward_mode == 'dynk_max'``, the input is on a ROCm device and the experts container is in its 'hip' mode,
@@ -17,7 +18,7 @@ from typing import Dict, Optional
 import torch
 from torch import nn
 
-from . import ops
+from . import functional, ops
 from .experts import MOE_IMPL_MAP, _HipContainer, _grad_wanted
 from .hip_abi import ACT
 
@@ -113,7 +114,58 @@ class MoeficationRouter(nn.Module):
         return x
 
 
+def route_topk_torch(logits, k, scoring='softmax', choice_bias=None, n_groups=1, kept_groups=1, group_score='top2',
+                     renormalise=True, scale=1.0):
+    """functional.route_topk composed in PyTorch, for tensors off the GPU: (routing, indices, weights), differentiable in the
+    logits.  The choice goes by float64 scores, as in the kernel, the weights are float32 (float64 for float64 logits)."""
+    n_experts = logits.size(-1)
+    z = logits.to(torch.promote_types(logits.dtype, torch.float32))
+    with torch.no_grad():
+        by = z.double()
+        bad = torch.isnan(by) | ((by == float('inf')) if scoring == 'softmax' else torch.zeros_like(by, dtype=torch.bool))
+        if choice_bias is not None or (n_groups > 1 and group_score == 'top2'):
+            # (softmax of a row without any finite logit: NaN, masked below)
+            by = torch.softmax(by, dim=-1) if scoring == 'softmax' else torch.sigmoid(by)
+            if choice_bias is not None:
+                by = by + choice_bias.double()
+        by = by.masked_fill(z == float('-inf'), float('-inf')) + 0.0
+        by = by.masked_fill((bad | torch.isnan(by)).any(dim=-1, keepdim=True), float('-inf'))
+        if n_groups > 1:
+            runs = by.unflatten(-1, (n_groups, n_experts // n_groups))
+            best = runs.sort(dim=-1, descending=True)[0][..., :2]
+            score = best[..., 0]
+            if group_score == 'top2' and best.size(-1) == 2:
+                score = score + best[..., 1].masked_fill(best[..., 1] == float('-inf'), 0.0)
+            dropped = score.sort(dim=-1, descending=True, stable=True)[1][..., kept_groups:]
+            out = torch.zeros_like(score, dtype=torch.bool).scatter_(-1, dropped, True)
+            by = runs.masked_fill(out.unsqueeze(-1), float('-inf')).flatten(-2)
+        by, order = by.sort(dim=-1, descending=True, stable=True)
+        there = by[..., :k] > float('-inf')
+        place = order[..., :k].masked_fill(~there, 0)
+        some = there.any(dim=-1, keepdim=True)
+    z = torch.where(some, z, 0.0)                              # a row that goes nowhere has no gradient either
+    at = z.gather(-1, place)
+    log_score = (at if renormalise else at - torch.logsumexp(z, dim=-1, keepdim=True)) if scoring == 'softmax' \
+        else nn.functional.logsigmoid(at)
+    log_score = torch.where(there, log_score, float('-inf'))
+    if renormalise:
+        weights = torch.softmax(torch.where(some, log_score, 0.0), dim=-1)
+    else:
+        weights = torch.exp(log_score)
+    weights = scale * torch.where(there, weights, 0.0)
+    target = place.masked_fill(~there, n_experts)              # places left over go to a column that is dropped
+    routing = torch.zeros(*z.shape[:-1], n_experts + 1, dtype=z.dtype, device=z.device).scatter(-1, target, weights)[..., :n_experts]
+    return routing.to(logits.dtype), place.masked_fill(~there, -1).to(torch.int32), weights
+
+
 class MoeficationMoE(MoELayer):
+    """The reference's layer (architectures/moe/moefication.py:28-101), with two gates of this package besides its four:
+    'softmax_topk' and 'sigmoid_topk' take the router's outputs as logits (a router with output_activation='identity') and
+    route every token to ``k`` experts with their scores as weights: softmax or sigmoid scores; ``balance_bias`` (float32
+    [E] or None) added for the choice only; the experts in ``n_groups`` runs of which ``kept_groups`` stay, scored by
+    ``group_score``; weights renormalised over the chosen when ``renormalise``, times ``route_scale``.  On a ROCm device this
+    is one HIP kernel with a backward pass of its own, so the router can be trained through the weights."""
+
     def __init__(self, name, hidden_dim, num_experts, bias, expert_dim, activation, experts_class='hip_kernel',
                  add_residual_connection=False, add_intermediate_gating=False):
         super().__init__(name, num_experts)
@@ -135,12 +187,20 @@ class MoeficationMoE(MoELayer):
         self.k = None
         self.tau = None
         self.add_residual_connection = add_residual_connection
+        # settings of the two gates by scores
+        self.register_buffer('balance_bias', None)   # absent from the state_dict until it is set
+        self.n_groups = self.kept_groups = 1
+        self.group_score = 'top2'
+        self.renormalise = True
+        self.route_scale = 1.0
         # Cost accounting (the reference sums (routing > 0) over the dense routing tensor on the host side of every
         # batch, eval.py:176-177): with collect_counts set, the fused HIP call also returns the per-expert number of
         # routed tokens from its own device-side counters; it stays on the device, nothing synchronises.
         self.collect_counts = False
         self._prepared = _CallCache()   # (key, ops.PreparedForward) of the fused call
         self.last_expert_counts: Optional[torch.Tensor] = None
+
+    SCORE_GATES = {'softmax_topk': 'softmax', 'sigmoid_topk': 'sigmoid'}
 
     # ------------------------------------------------------------------------------ gating
     def gate(self, x):
@@ -168,6 +228,19 @@ class MoeficationMoE(MoELayer):
             thresholds = max_norms * (1.0 - self.tau)
             routing = torch.zeros_like(norms)
             routing[norms >= thresholds] = 1.0
+            return routing
+        if mode in self.SCORE_GATES:
+            logits = self.router(x)
+            bias = None if self.balance_bias is None else self.balance_bias.float()
+            args = (self.k, self.SCORE_GATES[mode], bias, self.n_groups, self.kept_groups, self.group_score, self.renormalise,
+                    self.route_scale)
+            if logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16, torch.float16):
+                routing, _, _, counts = functional.route_topk(logits, *args, want_counts=self.collect_counts)
+                self.last_expert_counts = counts
+                return routing
+            routing, indices, _ = route_topk_torch(logits, *args)
+            self.last_expert_counts = torch.bincount(indices[indices >= 0].flatten(), minlength=self.num_experts).to(torch.int32) \
+                if self.collect_counts else None
             return routing
         raise ValueError(f'Unsupported forward_mode: {mode}')
 

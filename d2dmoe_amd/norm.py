@@ -1,0 +1,59 @@
+"""The models' layer norms with a HIP mode beside PyTorch's, chosen as the experts containers choose theirs: by
+``forward_mode``.
+
+``'torch'`` (the default) is ``F.layer_norm``, and the residual addition ahead of a block's second norm a tensor addition of
+its own.  ``'hip'`` runs the layer-norm kernels, forward and backward, with that addition inside (``add_norm``).  The two
+modes round alike at the tensors they store (the residual stream, the norm's output) and differ in the last bit of the
+latter at most."""
+from __future__ import annotations
+
+from torch import nn
+from torch.nn import functional as F
+
+from . import functional
+from .hip_abi import D2DMoEError
+
+
+class NormModes:
+    """Mixin of the layer-norm modules: `weight`, `bias` and `norm_eps()` come from the module."""
+    MODES = ('torch', 'hip')
+    forward_mode = 'torch'
+
+    def norm_eps(self) -> float:
+        return 1e-5
+
+    def _hip(self, x) -> bool:
+        if self.forward_mode not in self.MODES:
+            raise NotImplementedError(f'Unsupported forward_mode: {self.forward_mode}')
+        if self.forward_mode == 'torch':
+            return False
+        if not x.is_cuda:
+            raise D2DMoEError("forward_mode 'hip' needs a ROCm device; use 'torch' on the CPU")
+        return True
+
+    def forward(self, x, residual=None):
+        """norm(x), or (norm(x + residual), x + residual)."""
+        if self._hip(x):
+            return functional.layer_norm(x, self.weight, self.bias, self.norm_eps(), residual)
+        h = x if residual is None else x + residual
+        out = F.layer_norm(h, self.weight.shape, self.weight, self.bias, self.norm_eps())
+        return out if residual is None else (out, h)
+
+
+def add_norm(norm: nn.Module, x, residual):
+    """(norm(h), h) of the residual stream h = x + residual, where a block's next half begins.  In one call where the norm runs
+    on the HIP kernels; any other module sees the sum alone."""
+    if isinstance(norm, NormModes) and norm.forward_mode == 'hip':
+        return norm(x, residual)
+    h = x + residual
+    return norm(h), h
+
+
+def set_norm_mode(model: nn.Module, mode: str) -> int:
+    """Sets forward_mode of every layer norm of this package in `model`; returns how many there are."""
+    if mode not in NormModes.MODES:
+        raise ValueError(f'mode is one of {NormModes.MODES}, got {mode!r}')
+    norms = [m for m in model.modules() if isinstance(m, NormModes)]
+    for m in norms:
+        m.forward_mode = mode
+    return len(norms)

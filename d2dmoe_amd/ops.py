@@ -375,3 +375,153 @@ def forward(x: torch.Tensor, router_w1: Optional[torch.Tensor], router_w2: Optio
     prepared = PreparedForward(x.size(1), x.dtype, router_w1, router_w2, w1, b1, w2, w_up, last_bias, activation,
                                add_residual, packed, router_activation, router_output_activation)
     return prepared(x, thr_scale, norms_in, want_norms, want_counts, path, static_workspace, out, routing, norms, counts)
+
+
+# ---- layer norm and routing by scores --------------------------------------------------------------------------------
+def _launch(dev: torch.device, fn, what: str, *args) -> None:
+    """One library call on the tensors' device and that device's current stream."""
+    if dev.index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if status != 0:
+        abi.check(status, what)
+
+
+def _norm_params(what: str, d: int, dtype: torch.dtype, **params: Optional[torch.Tensor]) -> int:
+    """Element type code of weight and bias (the activations' type, or float32); both have to agree."""
+    kind = None
+    for name, p in params.items():
+        if p is None:
+            continue
+        if p.shape != (d,):
+            raise abi.D2DMoEError(f'{what}: {name} has shape {tuple(p.shape)}, the rows are {d} wide')
+        if p.dtype != dtype and p.dtype != torch.float32:
+            raise abi.D2DMoEError(f'{what}: {name} is {p.dtype}; with {dtype} activations it is {dtype} or torch.float32')
+        if kind is not None and p.dtype != kind:
+            raise abi.D2DMoEError(f'{what}: weight and bias are of two element types')
+        kind = p.dtype
+    return _DTYPES[dtype if kind is None else kind]
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               residual: Optional[torch.Tensor] = None, want_stats: bool = False):
+    """Layer norm of the rows of x [N,D], or of h = x + residual (rounded to the storage type), through d2dmoe_layer_norm.
+    Returns (out [N,D], h or None without a residual, mean, rstd): the last two float32 [N], or None without want_stats."""
+    code = _dtype_code(x)
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+        raise abi.D2DMoEError(f'layer_norm: residual is {residual.dtype} {tuple(residual.shape)}, x is {x.dtype} {tuple(x.shape)}')
+    if x.dim() != 2:
+        raise abi.D2DMoEError(f'layer_norm: x has {x.dim()} dimensions, the rows come as [N,D]')
+    dev = _require_gpu(x, residual, weight, bias)
+    lib = abi.load()
+    n, d = x.shape
+    pcode = _norm_params('layer_norm', d, x.dtype, weight=weight, bias=bias)
+    out = torch.empty_like(x)
+    total = None if residual is None else torch.empty_like(x)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=dev).unbind(0)
+    sh = abi.NormShape(n, d, code, pcode, eps)
+    _launch(dev, lib.d2dmoe_layer_norm, 'd2dmoe_layer_norm', ctypes.byref(sh), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
+            _ptr(total), out.data_ptr(), _ptr(mean), _ptr(rstd))
+    return out, total, mean, rstd
+
+
+def layer_norm_backward(grad_out: torch.Tensor, h: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                        rstd: torch.Tensor, grad_sum: Optional[torch.Tensor] = None, want_grad: bool = True,
+                        want_weight: bool = True, want_bias: bool = True, param_dtype: Optional[torch.dtype] = None):
+    """Gradients of layer_norm: (grad [N,D], that of x and of residual alike; grad_weight [D]; grad_bias [D]) through
+    d2dmoe_layer_norm_backward.  h, mean, rstd: what the forward call normalised (its x, or the sum it returned) and its
+    statistics; grad_sum: gradient of the returned sum.  The parameters' gradients have the weight's element type (without
+    a weight: param_dtype, by default the activations', and no grad_weight)."""
+    code = _dtype_code(h)
+    for name, t in (('grad_out', grad_out), ('grad_sum', grad_sum)):
+        if t is not None and (t.dtype != h.dtype or t.shape != h.shape):
+            raise abi.D2DMoEError(f'layer_norm_backward: {name} is {t.dtype} {tuple(t.shape)}, h is {h.dtype} {tuple(h.shape)}')
+    if h.dim() != 2:
+        raise abi.D2DMoEError(f'layer_norm_backward: h has {h.dim()} dimensions, the rows come as [N,D]')
+    n, d = h.shape
+    for name, t in (('mean', mean), ('rstd', rstd)):
+        if t.dtype != torch.float32 or t.shape != (n,):
+            raise abi.D2DMoEError(f'layer_norm_backward: {name} is {t.dtype} {tuple(t.shape)}, expected float32 ({n},)')
+    dev = _require_gpu(h, grad_out, grad_sum, weight, mean, rstd)
+    lib = abi.load()
+    pcode = _norm_params('layer_norm_backward', d, h.dtype, weight=weight)
+    ptype = weight.dtype if weight is not None else (param_dtype or h.dtype)
+    if weight is None:
+        if ptype != h.dtype and ptype != torch.float32:
+            raise abi.D2DMoEError(f'layer_norm_backward: param_dtype is {ptype}; with {h.dtype} activations it is that or torch.float32')
+        pcode = _DTYPES[ptype]
+    grad = torch.empty_like(h) if want_grad else None
+    gw = torch.empty(d, dtype=ptype, device=dev) if want_weight and weight is not None else None
+    gb = torch.empty(d, dtype=ptype, device=dev) if want_bias else None
+    if grad is None and gw is None and gb is None:
+        return None, None, None
+    sh = abi.NormShape(n, d, code, pcode, 0.0)
+    ws, nbytes = None, 0
+    if gw is not None or gb is not None:
+        # (a buffer of this call's own, not the one kept per stream: a captured call keeps its buffer with its graph)
+        nbytes = lib.d2dmoe_layer_norm_workspace_bytes(ctypes.byref(sh))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, lib.d2dmoe_layer_norm_backward, 'd2dmoe_layer_norm_backward', ctypes.byref(sh), grad_out.data_ptr(), _ptr(grad_sum),
+            h.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(grad), _ptr(gw), _ptr(gb), _ptr(ws), nbytes)
+    return grad, gw, gb
+
+
+def _route_shape(what: str, logits: torch.Tensor, k: int, scoring: str, renormalise: bool, scale: float, n_groups: int = 1,
+                 kept_groups: int = 1, group_score: str = 'top2') -> abi.RouteShape:
+    code = _dtype_code(logits)
+    if logits.dim() != 2:
+        raise abi.D2DMoEError(f'{what}: logits have {logits.dim()} dimensions, expected [N,E]')
+    if scoring not in abi.SCORING or group_score not in abi.GROUP_SCORE:
+        raise abi.D2DMoEError(f'{what}: scoring is one of {sorted(abi.SCORING)}, group_score one of {sorted(abi.GROUP_SCORE)}')
+    n, e = logits.shape
+    return abi.RouteShape(n, e, k, code, abi.SCORING[scoring], n_groups, kept_groups, abi.GROUP_SCORE[group_score],
+                          1 if renormalise else 0, scale)
+
+
+def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bias: Optional[torch.Tensor] = None,
+               n_groups: int = 1, kept_groups: int = 1, group_score: str = 'top2', renormalise: bool = True, scale: float = 1.0,
+               want_counts: bool = False):
+    """The k experts of every token and their weights from logits [N,E], through d2dmoe_route_topk.  Returns (routing [N,E]
+    with the weights at the chosen experts and 0 elsewhere, indices int32 [N,k] in descending order of choice, weights
+    float32 [N,k], counts int32 [E] or None); places left over hold index -1 and weight 0."""
+    sh = _route_shape('route_topk', logits, k, scoring, renormalise, scale, n_groups, kept_groups, group_score)
+    n, e = logits.shape
+    if choice_bias is not None and (choice_bias.dtype != torch.float32 or choice_bias.shape != (e,)):
+        raise abi.D2DMoEError(f'route_topk: choice_bias is {choice_bias.dtype} {tuple(choice_bias.shape)}, expected float32 ({e},)')
+    dev = _require_gpu(logits, choice_bias)
+    lib = abi.load()
+    routing = torch.empty_like(logits)
+    indices = torch.empty(n, max(k, 0), dtype=torch.int32, device=dev)
+    weights = torch.empty(n, max(k, 0), dtype=torch.float32, device=dev)
+    counts = torch.empty(e, dtype=torch.int32, device=dev) if want_counts else None
+    _launch(dev, lib.d2dmoe_route_topk, 'd2dmoe_route_topk', ctypes.byref(sh), logits.data_ptr(), _ptr(choice_bias),
+            routing.data_ptr(), indices.data_ptr(), weights.data_ptr(), _ptr(counts))
+    return routing, indices, weights, counts
+
+
+def route_topk_backward(logits: torch.Tensor, indices: torch.Tensor, scoring: str = 'softmax', renormalise: bool = True,
+                        scale: float = 1.0, grad_routing: Optional[torch.Tensor] = None,
+                        grad_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of the logits [N,E] from that of route_topk's routing and / or weights, through d2dmoe_route_topk_backward.
+    `indices` is what route_topk returned for these logits; scoring, renormalise and scale are that call's."""
+    if indices.dim() != 2 or indices.dtype != torch.int32 or indices.size(0) != logits.size(0):
+        raise abi.D2DMoEError(f'route_topk_backward: indices are {indices.dtype} {tuple(indices.shape)}, expected int32 [N,k]')
+    sh = _route_shape('route_topk_backward', logits, indices.size(1), scoring, renormalise, scale)
+    if grad_routing is None and grad_weights is None:
+        raise abi.D2DMoEError('route_topk_backward: pass grad_routing, grad_weights or both')
+    if grad_routing is not None and (grad_routing.dtype != logits.dtype or grad_routing.shape != logits.shape):
+        raise abi.D2DMoEError(f'route_topk_backward: grad_routing is {grad_routing.dtype} {tuple(grad_routing.shape)}, the logits are '
+                              f'{logits.dtype} {tuple(logits.shape)}')
+    if grad_weights is not None and (grad_weights.dtype != torch.float32 or grad_weights.shape != indices.shape):
+        raise abi.D2DMoEError(f'route_topk_backward: grad_weights is {grad_weights.dtype} {tuple(grad_weights.shape)}, expected float32 '
+                              f'{tuple(indices.shape)}')
+    dev = _require_gpu(logits, indices, grad_routing, grad_weights)
+    lib = abi.load()
+    grad = torch.empty_like(logits)
+    _launch(dev, lib.d2dmoe_route_topk_backward, 'd2dmoe_route_topk_backward', ctypes.byref(sh), logits.data_ptr(), indices.data_ptr(),
+            _ptr(grad_routing), _ptr(grad_weights), grad.data_ptr())
+    return grad

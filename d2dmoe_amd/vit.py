@@ -4,8 +4,9 @@ A plain VisionTransformer with the module tree and parameter names of torchvisio
 architectures/vit.py): `conv_proj`, `class_token`, `encoder.pos_embedding`, `encoder.layers.encoder_layer_<i>.{ln_1,
 self_attention, ln_2, mlp.0, mlp.3}`, `encoder.ln`, `heads.head` -- so a torchvision or reference state dict loads
 unchanged -- and the patched forwards that return the gating data of every MoE layer
-(architectures/moe/moe_models.py:55-78, 103-127).  Attention, LayerNorm, patch embedding and the head stay stock
-PyTorch; the FFNs become `MoeficationMoE` layers through `gpt2.replace_with_moes`, which recognises both backbones.
+(architectures/moe/moe_models.py:55-78, 103-127).  Attention, patch embedding and the head stay stock PyTorch, and so do
+the layer norms unless their `forward_mode` is 'hip' (`norm.set_norm_mode`); the FFNs become `MoeficationMoE` layers
+through `gpt2.replace_with_moes`, which recognises both backbones.
 """
 from __future__ import annotations
 
@@ -16,6 +17,14 @@ import torch
 from torch import nn
 
 from .layer import MoELayer
+from .norm import NormModes, add_norm
+
+
+class LayerNorm(NormModes, nn.LayerNorm):
+    """torch.nn.LayerNorm over the last dimension (same parameters); forward_mode 'hip' runs the HIP kernels (norm.py)."""
+
+    def norm_eps(self) -> float:
+        return self.eps
 
 
 class MLPBlock(nn.Sequential):
@@ -30,17 +39,17 @@ class EncoderBlock(nn.Module):
     def __init__(self, num_heads: int, hidden_dim: int, mlp_dim: int, dropout: float, attention_dropout: float):
         super().__init__()
         self.num_heads = num_heads
-        self.ln_1 = nn.LayerNorm(hidden_dim, eps=1e-6)
+        self.ln_1 = LayerNorm(hidden_dim, eps=1e-6)
         self.self_attention = nn.MultiheadAttention(hidden_dim, num_heads, dropout=attention_dropout, batch_first=True)
         self.dropout = nn.Dropout(dropout)
-        self.ln_2 = nn.LayerNorm(hidden_dim, eps=1e-6)
+        self.ln_2 = LayerNorm(hidden_dim, eps=1e-6)
         self.mlp = MLPBlock(hidden_dim, mlp_dim, dropout)
 
     def forward(self, input: torch.Tensor):
         x = self.ln_1(input)
         x, _ = self.self_attention(x, x, x, need_weights=False)
-        x = self.dropout(x) + input
-        return x + self.mlp(self.ln_2(x))
+        y, x = add_norm(self.ln_2, self.dropout(x), input)
+        return x + self.mlp(y)
 
 
 class Encoder(nn.Module):
@@ -51,7 +60,7 @@ class Encoder(nn.Module):
         self.layers = nn.Sequential(OrderedDict(
             (f'encoder_layer_{i}', EncoderBlock(num_heads, hidden_dim, mlp_dim, dropout, attention_dropout))
             for i in range(num_layers)))
-        self.ln = nn.LayerNorm(hidden_dim, eps=1e-6)
+        self.ln = LayerNorm(hidden_dim, eps=1e-6)
 
     def forward(self, input: torch.Tensor):
         return self.ln(self.layers(self.dropout(input + self.pos_embedding)))
@@ -90,8 +99,7 @@ def moe_vit_block_forward(self, input: torch.Tensor):
     gating_data = {}
     x = self.ln_1(input)
     x, _ = self.self_attention(x, x, x, need_weights=False)
-    x = self.dropout(x) + input
-    y = self.ln_2(x)
+    y, x = add_norm(self.ln_2, self.dropout(x), input)
     if isinstance(self.mlp, MoELayer):
         y, ffn_gating_data = self.mlp(y)
         gating_data.update(ffn_gating_data)

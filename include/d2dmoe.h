@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define D2DMOE_VERSION 211 /* major*10000 + minor*100 + patch */
+#define D2DMOE_VERSION 300 /* major*10000 + minor*100 + patch */
 
 /* status codes */
 enum {
@@ -47,8 +47,9 @@ enum {
   D2DMOE_E_UNSUPPORTED = -6, /* valid request that this build has no kernel for */
   D2DMOE_E_ALIGN = -7,       /* a tensor pointer is not aligned to 16 bytes */
   D2DMOE_E_STATIC_LIMIT = -8, /* d2dmoe_forward_static: the shape needs more than D2DMOE_STATIC_WORKSPACE_BYTES of workspace */
-  D2DMOE_E_PACKED = -9       /* a packed buffer came without its descriptor, or the descriptor says it was packed for another
+  D2DMOE_E_PACKED = -9,      /* a packed buffer came without its descriptor, or the descriptor says it was packed for another
                                 layer (shape, element type, sections) or by another layout version */
+  D2DMOE_E_VALUE = -10       /* a scalar argument (eps, scale, scoring, ...) is outside its range */
 };
 
 /* element types */
@@ -289,6 +290,77 @@ int d2dmoe_pack_norms(const d2dmoe_shape* shape, const void* w1, const void* b1,
                       void* packed, size_t packed_bytes, void* stream);
 int d2dmoe_expert_output_norms(const d2dmoe_shape* shape, const void* x, const void* packed, void* norms,
                                void* stream);
+
+/* ---- layer norm --------------------------------------------------------------------------------------------------
+ * Rows of h = x, or of h = x + residual rounded to T (the residual stream between a block's two halves):
+ *   m = mean(h)   v = mean((h - m)^2)   r = 1 / sqrt(v + eps)   out = (h - m) r * weight + bias
+ * Replaces the LayerNorm modules in front of a block's attention and FFN (architectures/gpt.py:27-36, 117-128) together
+ * with the residual addition ahead of the second one.  Statistics, sums and intermediates are float32; every stored
+ * value is rounded once.  Any width, any element-aligned pointer.  Nothing may overlap an output. */
+typedef struct d2dmoe_norm_shape {
+  int64_t n_rows;       /* >= 0 */
+  int32_t width;        /* 1 .. 2^24 */
+  int32_t dtype;        /* x, residual, sum, out and their gradients */
+  int32_t param_dtype;  /* weight, bias and their gradients: dtype, or D2DMOE_F32 */
+  float eps;            /* finite, >= 0 */
+} d2dmoe_norm_shape;
+
+/*   residual optional [n_rows,width]; sum optional: receives h (with a residual); weight, bias optional [width]
+ *   mean, rstd optional float32 [n_rows]: the row statistics, what the backward pass needs next to h */
+int d2dmoe_layer_norm(const d2dmoe_norm_shape* shape, const void* x, const void* residual, const void* weight, const void* bias,
+                      void* sum, void* out, float* mean, float* rstd, void* stream);
+
+/* Backward: with n = (h - m) r and u = grad_out * weight,
+ *   grad = r (u - mean(u) - n mean(u n)) + grad_sum       the gradient of x and of residual alike
+ *   grad_weight = sum over rows of grad_out n             grad_bias = sum over rows of grad_out
+ *   h: what the forward pass normalised (its x, or its `sum`); grad_sum optional: gradient of `sum` from its other uses
+ *   grad, grad_weight, grad_bias optional each (grad_weight and grad_bias of no rows are zero)
+ * The row sums are added in a fixed order: same inputs, same bits.
+ * workspace: d2dmoe_layer_norm_workspace_bytes(shape), 256-byte aligned, needed for grad_weight and grad_bias only. */
+size_t d2dmoe_layer_norm_workspace_bytes(const d2dmoe_norm_shape* shape);
+int d2dmoe_layer_norm_backward(const d2dmoe_norm_shape* shape, const void* grad_out, const void* grad_sum, const void* h,
+                               const void* weight, const float* mean, const float* rstd, void* grad, void* grad_weight,
+                               void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- routing by scores -------------------------------------------------------------------------------------------
+ * The k experts of a token from a learned router's logits z, with weights: next to d2dmoe_select's dynamic-k rule, the
+ * fixed-k rule of trained mixtures (and the weighted form of the reference's 'topk' gate, moefication.py:63-69).
+ *   scores  s = softmax(z) or 1 / (1 + exp(-z))
+ *   choice  c = s + choice_bias[e]; c = z where there is no bias and no sum of scores is needed (same order)
+ *   groups  n_groups runs of n_experts / n_groups consecutive experts, a run scored by its largest c or by the sum of its
+ *           two largest; the kept_groups best runs stay (ties: the lowest run)
+ *   chosen  the k largest c that remain, in descending order, ties to the lowest index.  An expert with z = -inf is never
+ *           chosen; a row with a NaN among its c (softmax: also with z = +inf) chooses nothing, as d2dmoe_select's rows do
+ *   weights w = scale * s, or scale * s / (sum of the chosen s)
+ * The choice is made on float64 scores, the weights are float32. */
+enum { D2DMOE_SCORE_SOFTMAX = 0, D2DMOE_SCORE_SIGMOID = 1 };
+enum { D2DMOE_GROUP_MAX = 0, D2DMOE_GROUP_TOP2 = 1 };
+typedef struct d2dmoe_route_shape {
+  int64_t n_tokens;     /* >= 0 */
+  int32_t n_experts;    /* 1 .. 1024 */
+  int32_t k;            /* 1 .. kept_groups * (n_experts / n_groups) */
+  int32_t dtype;        /* logits, routing and their gradients */
+  int32_t scoring;      /* D2DMOE_SCORE_* */
+  int32_t n_groups;     /* divides n_experts; 1: no groups */
+  int32_t kept_groups;  /* 1 .. n_groups */
+  int32_t group_score;  /* D2DMOE_GROUP_* (read with n_groups > 1) */
+  int32_t renormalise;  /* 1: the chosen weights of a row add up to scale */
+  float scale;          /* finite */
+} d2dmoe_route_shape;
+
+/*   choice_bias optional float32 [n_experts]
+ *   routing optional T [n_tokens,n_experts]: the weights as the dense routing tensor every experts entry point takes
+ *   indices optional int32 [n_tokens,k], weights optional float32 [n_tokens,k]: the same by place (-1 and 0 where a place is
+ *   left over)      counts optional int32 [n_experts]: tokens per expert (zeroed here) */
+int d2dmoe_route_topk(const d2dmoe_route_shape* shape, const void* logits, const float* choice_bias, void* routing,
+                      int32_t* indices, float* weights, int32_t* counts, void* stream);
+
+/* Gradient of the logits from the gradient of the weights, given by expert (grad_routing T [n_tokens,n_experts], read at the
+ * chosen experts), by place (grad_weights float32 [n_tokens,k]), or both (added).  indices: what the forward pass wrote
+ * (an index outside 0 .. n_experts - 1 counts as a place left over).  The choice itself has no gradient, so the bias and
+ * the groups do not enter: n_groups, kept_groups and group_score are not read. */
+int d2dmoe_route_topk_backward(const d2dmoe_route_shape* shape, const void* logits, const int32_t* indices,
+                               const void* grad_routing, const float* grad_weights, void* grad_logits, void* stream);
 
 #ifdef __cplusplus
 }

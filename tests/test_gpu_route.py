@@ -1,0 +1,379 @@
+"""Routing by scores on the GPU against the float64 oracle: indices equal, weights and gradients within float32 rounding.
+
+Tolerances.  u = 2^-24.  A weight is exp of a difference (argument rounded: u |argument| relative, arguments up to 2 max|z|), a
+sum of at most E terms in a tree over lanes with chains of at most 16, a division and a product: relative error at most
+u (2 max|z| + 64).  A routing entry is that, rounded once to the storage type.  A gradient is a product of a weight with a
+difference of gradients, each of whose terms carries that error."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import norm_route as R
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda:0'
+U = 2.0 ** -24
+
+
+def _ops():
+    from d2dmoe_amd import ops
+    return ops
+
+
+def _half(t):
+    return torch.finfo(t).eps / 2
+
+
+def _logits(n, e, t, seed, ties=False, masks=False):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(n, e, generator=g) * 1.5 + torch.randn(e, generator=g) * 0.5
+    if ties:
+        z = (z * 2).round() / 2
+    if masks:
+        z[torch.rand(n, e, generator=g) < 0.2] = -math.inf
+        z[::7] = -math.inf                                # rows that a padding mask emptied
+        z[3::11, e // 2] = math.nan
+        z[5::13, 0] = math.inf
+        z[4::17] = torch.finfo(t).min                     # masked with the type's lowest value: ordinary, equal logits
+    return z.to(t)
+
+
+def _check(z, k, scoring, bias, kw, t, got):
+    routing, indices, weights, counts = got
+    want, idx, w = R.route(z.double().numpy(), k, scoring, bias=None if bias is None else bias.double().numpy(), **kw)
+    assert indices.dtype == torch.int32 and np.array_equal(indices.cpu().numpy(), idx)
+    big = z.float()[torch.isfinite(z.float()) & (z.float() > -1e4)]
+    tol = U * (2 * big.abs().max().item() + 64 if big.numel() else 64)
+    err = np.abs(weights.double().cpu().numpy() - w)
+    assert weights.dtype == torch.float32 and (err <= tol * w + 1e-37).all(), (err / (w + 1e-37)).max()
+    err = np.abs(routing.double().cpu().numpy() - want)
+    assert routing.dtype == t and (err <= (tol + _half(t)) * want + 2.0 ** -25 * (t == torch.float16) + 1e-37).all()
+    if counts is not None:
+        assert np.array_equal(counts.cpu().numpy(), np.bincount(idx[idx >= 0], minlength=z.size(1)))
+    return idx, tol
+
+
+def _check_grad(z, idx, q, scoring, renormalise, scale, t, grad, tol):
+    zz = z.double().numpy()
+    want = R.route_grads(zz, idx, q, scoring, renormalise, scale)
+    # every term is a product of scores (<= 1) with gradients; the row's largest gradient bounds the terms that cancel
+    size = np.abs(q).max(1, initial=0.0)[:, None] * scale
+    if renormalise:
+        w = R.route_grads(zz, idx, np.ones_like(q), scoring, False, 1.0)    # where a gradient can be at all
+        bound = 4 * tol * size * (np.abs(want) + np.abs(w) > 0)
+    else:
+        bound = 4 * tol * size
+    err = np.abs(grad.double().cpu().numpy() - want)
+    assert grad.dtype == t and (err <= bound + _half(t) * np.abs(want) + 2.0 ** -25 * (t == torch.float16)).all(), (err - bound).max()
+
+
+EXPERTS = [1, 2, 3, 7, 8, 24, 60, 64, 65, 100, 128, 129, 160, 256, 320, 512, 513, 1000, 1024]
+
+
+@pytest.mark.parametrize('t', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('e', EXPERTS)
+def test_plain_choice(e, t):
+    for k in sorted({1, 2, 8, min(e, 33), e if e <= 129 else 70}):
+        if k > e:
+            continue
+        for scoring in ('softmax', 'sigmoid'):
+            for renormalise in (True, False):
+                print('route', e, k, t, scoring, renormalise, flush=True)
+                z = _logits(29, e, t, seed=e + k, ties=k % 2 == 0, masks=True)
+                kw = dict(renormalise=renormalise, scale=1.0 if renormalise else 2.5)
+                got = _ops().route_topk(z.to(DEV), k, scoring, want_counts=True, **kw)
+                idx, tol = _check(z, k, scoring, None, kw, t, got)
+                g = torch.Generator().manual_seed(k)
+                q, dense = torch.randn(29, k, generator=g), torch.randn(29, e, generator=g).to(t)
+                grad = _ops().route_topk_backward(z.to(DEV), got[1], scoring, grad_weights=q.to(DEV), **kw)
+                _check_grad(z, idx, q.double().numpy(), scoring, renormalise, kw['scale'], t, grad, tol)
+                by_place = np.where(idx >= 0, np.take_along_axis(dense.double().numpy(), np.maximum(idx, 0), 1), 0.0)
+                grad = _ops().route_topk_backward(z.to(DEV), got[1], scoring, grad_routing=dense.to(DEV), **kw)
+                _check_grad(z, idx, by_place, scoring, renormalise, kw['scale'], t, grad, tol)
+                grad = _ops().route_topk_backward(z.to(DEV), got[1], scoring, grad_routing=dense.to(DEV), grad_weights=q.to(DEV), **kw)
+                _check_grad(z, idx, by_place + q.double().numpy(), scoring, renormalise, kw['scale'], t, grad, tol)
+
+
+@pytest.mark.parametrize('t', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('e,groups,kept,k', [(8, 2, 1, 3), (8, 4, 2, 4), (8, 8, 3, 2), (12, 3, 2, 5), (24, 3, 1, 8), (60, 5, 2, 6), (64, 8, 4, 8),
+                                             (96, 8, 3, 6), (128, 4, 2, 8), (128, 64, 9, 8), (160, 8, 3, 6), (256, 8, 4, 8), (256, 1, 1, 8),
+                                             (320, 10, 5, 8), (512, 2, 1, 4), (512, 16, 4, 12), (1000, 10, 4, 8), (1024, 32, 4, 8),
+                                             (1024, 1024, 40, 33)])
+def test_groups_and_bias(e, groups, kept, k, t):
+    for scoring in ('softmax', 'sigmoid'):
+        for score in ('top2', 'max'):
+            for biased in (True, False):
+                print('groups', e, groups, kept, k, t, scoring, score, biased, flush=True)
+                z = _logits(23, e, t, seed=e + groups, ties=score == 'max', masks=True)
+                bias = torch.randn(e, generator=torch.Generator().manual_seed(3)) * (0.1 if scoring == 'sigmoid' else 0.5 / e) if biased else None
+                if biased and e > 8:
+                    bias[1] = -math.inf                  # an expert the bias switches off
+                kw = dict(n_groups=groups, kept_groups=kept, group_score=score, renormalise=True, scale=2.5)
+                got = _ops().route_topk(z.to(DEV), k, scoring, None if bias is None else bias.to(DEV), want_counts=True, **kw)
+                _check(z, k, scoring, bias, kw, t, got)
+
+
+def test_bias_that_is_not_a_number_routes_nothing():
+    z = _logits(9, 32, torch.float32, seed=1)
+    bias = torch.zeros(32)
+    bias[4] = math.nan
+    routing, indices, weights, counts = _ops().route_topk(z.to(DEV), 4, 'sigmoid', bias.to(DEV), want_counts=True)
+    assert (indices == -1).all() and not routing.any() and not weights.any() and not counts.any()
+
+
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+def test_neighbours_that_float32_scores_do_not_tell_apart(scoring):
+    """Choices whose difference lies below float32's step at the score: pairs of experts whose scores plus bias differ by a few
+    2^-40 (the bias takes back what the logits differ by, up to its own rounding), in every row."""
+    g = torch.Generator().manual_seed(6)
+    z = torch.randn(4000, 64, generator=g)
+    z = z + 0.0
+    z[:, 1::2] = z[:, ::2]                               # equal pairs ...
+    z[:, 1::2] *= 1 + 2.0 ** -22                         # ... a step or two apart
+    bias = torch.full((64,), 0.25)
+    for k, kw in ((8, {}), (6, dict(n_groups=8, kept_groups=3, group_score='top2')), (6, dict(n_groups=8, kept_groups=3, group_score='max'))):
+        got = _ops().route_topk(z.to(DEV), k, scoring, bias.to(DEV), **kw)
+        _check(z[:400], k, scoring, bias, kw, torch.float32, (got[0][:400], got[1][:400], got[2][:400], None))
+    # zero bias, 16-bit logits: ties in nearly every row
+    zb = z.bfloat16()
+    got = _ops().route_topk(zb.to(DEV), 8, scoring, torch.zeros(64, device=DEV))
+    _check(zb[:400], 8, scoring, torch.zeros(64), {}, torch.bfloat16, (got[0][:400], got[1][:400], got[2][:400], None))
+
+
+def test_scores_that_underflow_still_share_their_weight():
+    """Chosen scores of 1e-60 and less: renormalised weights go by their ratio."""
+    z = torch.tensor([[-140.0, -139.0, -150.0, -400.0], [-3e38, -3e38, -3e38, -3e38]])
+    for scoring in ('softmax', 'sigmoid'):
+        got = _ops().route_topk(z.to(DEV), 2, scoring)
+        # (row 1: equal logits; the arguments are differences of the logits, so the bound of the other tests holds)
+        assert got[1].tolist() == [[1, 0], [0, 1]]
+        want = [[1 / (1 + math.exp(-1)), 1 / (1 + math.exp(1))], [0.5, 0.5]]
+        assert np.abs(got[2].cpu().numpy() - want).max() < 64 * U
+    # a bias that chooses experts far below the row's best
+    bias = torch.tensor([0.0, 0.0, 5.0, 6.0])
+    got = _ops().route_topk(torch.tensor([[0.0, 1.0, -200.0, -201.0]], device=DEV), 2, 'softmax', bias.to(DEV))
+    assert got[1].tolist() == [[3, 2]] and abs(got[2][0, 1].item() - 1 / (1 + math.exp(-1))) < 64 * U
+
+
+def test_no_tokens_and_many():
+    ops = _ops()
+    e = torch.empty(0, 16, device=DEV)
+    routing, indices, weights, counts = ops.route_topk(e, 3, want_counts=True)
+    assert routing.shape == (0, 16) and indices.shape == weights.shape == (0, 3) and not counts.any()
+    assert ops.route_topk_backward(e, indices, grad_weights=weights).shape == (0, 16)
+    # more than 2^31 logits
+    n = (1 << 21) + 5
+    z = torch.zeros(n, 1024, dtype=torch.bfloat16, device=DEV)
+    tail = _logits(5, 1024, torch.bfloat16, seed=4)
+    z[-5:] = tail.to(DEV)
+    routing, indices, weights, _ = ops.route_topk(z, 4)
+    _check(tail, 4, 'softmax', None, {}, torch.bfloat16, (routing[-5:], indices[-5:], weights[-5:], None))
+    assert (indices[:-5] == torch.arange(4, device=DEV)).all() and (weights[:-5] == 0.25).all()
+    q = torch.ones(n, 4, device=DEV)
+    q[-5:, 0] = 2.0
+    grad = ops.route_topk_backward(z, indices, grad_weights=q)
+    assert not grad[:-5].any() and grad[-5:].any()
+    del z, routing, grad
+
+
+def test_places_that_are_no_experts_are_left_out():
+    """Indices of the caller's own making: out of range counts as left over, the same expert twice adds up."""
+    z = _logits(6, 40, torch.float32, seed=2)
+    idx = torch.tensor([[3, -1, 7], [40, 5, 2], [1 << 30, -5, 0], [9, 9, 4], [-1, -1, -1], [39, 0, 38]], dtype=torch.int32)
+    q = torch.randn(6, 3, generator=torch.Generator().manual_seed(1))
+    for scoring in ('softmax', 'sigmoid'):
+        for renormalise in (True, False):
+            grad = _ops().route_topk_backward(z.to(DEV), idx.to(DEV), scoring, renormalise, 1.5, grad_weights=q.to(DEV))
+            _check_grad(z, idx.numpy(), q.double().numpy(), scoring, renormalise, 1.5, torch.float32, grad, U * 80)
+
+
+@pytest.mark.parametrize('off', [1, 3])
+def test_rows_that_start_anywhere_and_bytes_around_them(off):
+    import ctypes
+    from d2dmoe_amd import hip_abi as abi
+    lib = abi.load()
+    for t, code in ((torch.bfloat16, abi.BF16), (torch.float32, abi.F32)):
+        for n, e, k in ((7, 128, 8), (9, 60, 5), (5, 31, 31), (3, 700, 20)):
+            z = _logits(n, e, t, seed=n)
+            q = torch.randn(n, e, generator=torch.Generator().manual_seed(7)).to(t)
+
+            def place(v):
+                buf = torch.full((off + v.numel() + 64,), 7.0, dtype=v.dtype, device=DEV)
+                buf[off:off + v.numel()] = v.reshape(-1).to(DEV)
+                return buf
+
+            ins = [place(z), place(q)]
+            outs = [torch.full((off + c + 64,), 7, dtype=ty, device=DEV) for c, ty in
+                    ((n * e, t), (n * k, torch.int32), (n * k, torch.float32), (e, torch.int32), (n * e, t))]
+            at = [v.data_ptr() + off * v.element_size() for v in ins + outs]
+            rs = abi.RouteShape(n, e, k, code, 0, 1, 1, 0, 1, 1.0)
+            s = torch.cuda.current_stream().cuda_stream
+            abi.check(lib.d2dmoe_route_topk(ctypes.byref(rs), at[0], None, at[2], at[3], at[4], at[5], s), 'forward')
+            abi.check(lib.d2dmoe_route_topk_backward(ctypes.byref(rs), at[0], at[3], at[1], None, at[6], s), 'backward')
+            sizes = (n * e, n * k, n * k, e, n * e)
+            for v, c in zip(outs, sizes):
+                assert (v[:off] == 7).all() and (v[off + c:] == 7).all()
+            cut = [v[off:off + c] for v, c in zip(outs, sizes)]
+            idx, tol = _check(z, k, 'softmax', None, {}, t, (cut[0].view(n, e), cut[1].view(n, k), cut[2].view(n, k), cut[3]))
+            by_place = np.take_along_axis(q.double().numpy(), idx, 1)
+            _check_grad(z, idx, by_place, 'softmax', True, 1.0, t, cut[4].view(n, e), tol)
+            # each output alone
+            alone = torch.full_like(outs[1], 7)
+            abi.check(lib.d2dmoe_route_topk(ctypes.byref(rs), at[0], None, None, alone.data_ptr() + off * 4, None, None, s), 'indices')
+            assert torch.equal(alone, outs[1])
+
+
+def test_on_a_stream_of_its_own_and_captured():
+    ops = _ops()
+    cases = []
+    for seed, (n, e) in enumerate(((900, 128), (500, 320))):
+        z = _logits(n, e, torch.bfloat16, seed=seed).to(DEV)
+        q = torch.randn(n, e, generator=torch.Generator().manual_seed(seed)).bfloat16().to(DEV)
+        bias = torch.randn(e, device=DEV) * 0.05
+
+        def step(z=z, q=q, bias=bias):
+            routing, indices, weights, counts = ops.route_topk(z, 6, 'sigmoid', bias, want_counts=True)
+            return routing, indices, weights, counts, ops.route_topk_backward(z, indices, 'sigmoid', grad_routing=q)
+
+        eager = [v.clone() for v in step()]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for a, c in zip(step(), eager):
+                assert torch.equal(a, c)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        cases.append((graph, got, eager, step))
+    for _ in range(4):
+        for graph, got, eager, step in cases:
+            for v in got:
+                v.fill_(3)
+            graph.replay()
+            step()
+            torch.cuda.synchronize()
+            for a, c in zip(got, eager):
+                assert torch.equal(a, c)
+
+
+def test_gradient_is_the_difference_quotient():
+    """float32, central differences of step 2^-7 of the weights' sum with q: truncation 2^-14 / 6 of a third derivative of order
+    one, rounding 2^-24 of weights below 2.5 over the step (4e-5)."""
+    ops = _ops()
+    z = _logits(3, 20, torch.float32, seed=12).to(DEV)
+    q = torch.randn(3, 4, generator=torch.Generator().manual_seed(2)).to(DEV)
+    step = 2.0 ** -7
+    for scoring in ('softmax', 'sigmoid'):
+        for renormalise in (True, False):
+            _, idx, _, _ = ops.route_topk(z, 4, scoring, renormalise=renormalise, scale=2.5)
+            grad = ops.route_topk_backward(z, idx, scoring, renormalise, 2.5, grad_weights=q)
+            for j in range(20):
+                sums = []
+                for sign in (1, -1):
+                    v = z.clone()
+                    v[:, j] += sign * step
+                    _, i2, w2, _ = ops.route_topk(v, 20, scoring, renormalise=False, scale=1.0)
+                    s = torch.zeros_like(z).scatter_(1, i2.long(), w2).gather(1, idx.long()).double()      # scores of the same experts
+                    w = 2.5 * (s / s.sum(1, keepdim=True) if renormalise else s)
+                    sums.append((w * q.double()).sum(1))
+                quotient = (sums[0] - sums[1]) / (2 * step)
+                assert (quotient - grad[:, j].double()).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize('t', [torch.float32, torch.bfloat16])
+def test_differentiable_function_and_layer(t):
+    """The MoE layer's gates by scores: routing equal to the composition in PyTorch, router gradients through both experts modes
+    that can be trained, and the weighted routing honoured by the HIP experts."""
+    from d2dmoe_amd import MoeficationMoE, MoeficationRouter, functional
+    from d2dmoe_amd.layer import route_topk_torch
+    torch.manual_seed(3)
+    moe = MoeficationMoE('m', 256, 32, True, 16, torch.nn.ReLU)
+    moe.router = MoeficationRouter(256, 32, width=64, depth=2, activation='relu', output_activation='identity')
+    moe = moe.to(DEV).to(t)
+    x = torch.randn(3, 50, 256, device=DEV).to(t)
+    moe.k, moe.collect_counts = 5, True
+    for mode, scoring in (('softmax_topk', 'softmax'), ('sigmoid_topk', 'sigmoid')):
+        moe.forward_mode = mode
+        moe.n_groups, moe.kept_groups = (4, 2) if scoring == 'sigmoid' else (1, 1)
+        moe.balance_bias = 0.05 * torch.randn(32, device=DEV) if scoring == 'sigmoid' else None
+        logits = moe.router(x)
+        bias = None if moe.balance_bias is None else moe.balance_bias.float()
+        args = (5, scoring, bias, moe.n_groups, moe.kept_groups)
+        routing, indices, weights, counts = functional.route_topk(logits, *args, want_counts=True)
+        ref, ref_idx, ref_w = route_topk_torch(logits, *args)
+        assert indices.shape == weights.shape == (3, 50, 5) and torch.equal(indices, ref_idx)
+        assert (weights - ref_w).abs().max() <= 128 * U
+        q, g = torch.randn_like(weights), torch.randn_like(routing)
+        a = torch.autograd.grad((routing, weights), logits, (g, q), retain_graph=True)[0]
+        c = torch.autograd.grad((ref, ref_w), logits, (g, q), retain_graph=True)[0]
+        # the composition rounds routing's gradient and the sum of the two once more
+        assert (a - c).abs().max() <= 4 * _half(t) * c.abs().max() + 1e-5
+        assert torch.equal(counts.long(), torch.bincount(indices.flatten().long(), minlength=32))
+        # the layer: masked experts train, HIP experts answer; both see the same weighted routing
+        moe.experts.forward_mode = 'masked'
+        out, gating = moe(x)
+        out.float().square().mean().backward()
+        grad = moe.router.layers[0].weight.grad
+        assert torch.isfinite(grad).all() and grad.abs().sum() > 0
+        assert torch.equal(moe.last_expert_counts.long(), (gating['m'][0] != 0).sum((0, 1)))
+        moe.zero_grad()
+        moe.experts.forward_mode = 'hip'
+        with torch.no_grad():
+            moe.router_logits = None
+            got, gating2 = moe(x)
+            want = moe.experts.forward_all(x.view(-1, 256).double() if t == torch.float64 else x.view(-1, 256),
+                                           gating2['m'][0].view(-1, 32)) + moe.last_bias
+        err = (got.view(-1, 256).float() - want.float()).abs().max() / want.float().abs().max()
+        assert err < (1e-5 if t == torch.float32 else 2e-2)
+
+
+def test_together_as_a_block_uses_them():
+    """GPT-2 with expert layers routed by scores and every norm on the HIP kernels: one training step in float32 against the same
+    model composed in PyTorch, then the served model (norm, router, choice, weighted experts all on the HIP kernels)."""
+    from d2dmoe_amd import add_routers, gpt2, set_norm_mode
+    from d2dmoe_amd.layer import route_topk_torch
+    import d2dmoe_amd.layer as layer_module
+    torch.manual_seed(5)
+    base = gpt2.GPT(gpt2.GPTConfig(block_size=64, vocab_size=128, n_layer=2, n_head=4, n_embd=256))
+    moe, names = gpt2.replace_with_moes(base, num_experts=16)
+    gpt2.split_original_parameters(base, moe, names)
+    add_routers(moe, dict(width=64, depth=2, bias=False, activation='relu', output_activation='identity'))
+    moe = moe.to(DEV)
+    idx = torch.randint(0, 128, (2, 64), device=DEV)
+    layers = [gpt2.get_module_by_name(moe, n) for n in names]
+    for lay in layers:
+        lay.forward_mode, lay.k = 'softmax_topk', 4
+        lay.experts.forward_mode = 'masked'
+
+    def step():
+        moe.zero_grad()
+        logits = moe(idx)
+        torch.nn.functional.cross_entropy(logits.view(-1, 128).float(), idx.roll(-1, 1).view(-1)).backward()
+        return logits.detach().clone(), {k: v.grad.clone() for k, v in moe.named_parameters() if v.grad is not None}
+
+    set_norm_mode(moe, 'hip')
+    hip = step()
+    kept = functional_route = layer_module.functional.route_topk
+    try:
+        layer_module.functional.route_topk = lambda z, *a, want_counts=False: (*route_topk_torch(z, *a), None)
+        set_norm_mode(moe, 'torch')
+        plain = step()
+    finally:
+        layer_module.functional.route_topk = kept
+    assert functional_route is kept
+    assert (hip[0] - plain[0]).abs().max() <= 1e-4 * plain[0].abs().max()
+    assert set(hip[1]) == set(plain[1]) and any('router' in k for k in hip[1])
+    for k in plain[1]:
+        assert (hip[1][k] - plain[1][k]).norm() <= 1e-3 * plain[1][k].norm() + 1e-9, k
+    # served: everything on the HIP kernels
+    set_norm_mode(moe, 'hip')
+    for lay in layers:
+        lay.experts.forward_mode = 'hip'
+    with torch.no_grad():
+        served, gating = moe(idx, return_gating_data=True)
+    assert (served - plain[0]).abs().max() <= 1e-4 * plain[0].abs().max()
+    assert all(((g[0] > 0).sum(-1) == 4).all() for g in gating.values())
