@@ -36,7 +36,458 @@ __device__ inline float wave_max(float v) {
 }
 __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 
-// One wave per token.
+// =====================================================================================================
+// Teams: L lanes per token, 64 / L tokens per wave, V consecutive experts per lane (L V >= E, L >= k).
+//
+// A row is read once, as one or two 16-byte loads per lane.  Each lane sorts its V keys (choice, then lowest index: 64 bits
+// that compare as unsigned numbers); the k best are then the team's largest list head, taken k times: two maxima over the
+// team (value, then index) in lane-permute instructions, and the winner's list moves up by one.  Place i ends in lane i, which
+// computes its weight; the dense row goes through a zeroed LDS tile of the wave's tokens, so that it leaves as whole 16-byte
+// stores.  Waves share nothing, so there are no barriers.
+//
+// Choices that are not the logits themselves are made on float32 scores first, whose error is below 12 u (u = 2^-24: exp, sum,
+// division, one addition; a score is at most 1) plus u |c|.  Where two choices whose order matters lie within 2^-19 + 2^-22 |c|
+// of each other -- places next to one another in the list, the last place and the first one left out, a group that stays and
+// one that goes -- the wave repeats its choice on float64 scores; a row or two in a thousand do.
+// =====================================================================================================
+constexpr int WAVES = 4;   // per workgroup
+
+template <int CTRL>
+__device__ inline uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+
+// All-reduce over aligned teams of L lanes: neighbours, pairs, quads (mirror of 8), eights (mirror of 16), rows, halves.
+template <int L, typename Op>
+__device__ inline uint32_t team_reduce(uint32_t v, Op op) {
+  if constexpr (L >= 2) v = op(v, dpp<0xB1>(v));
+  if constexpr (L >= 4) v = op(v, dpp<0x4E>(v));
+  if constexpr (L >= 8) v = op(v, dpp<0x141>(v));
+  if constexpr (L >= 16) v = op(v, dpp<0x140>(v));
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  return v;
+}
+template <int L>
+__device__ inline uint32_t team_max_u(uint32_t v) { return team_reduce<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
+template <int L>
+__device__ inline float team_max(float v) {
+  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int L>
+__device__ inline float team_sum(float v) {
+  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+template <int L>
+__device__ inline double team_sum(double v) {
+#pragma unroll
+  for (int off = 1; off < L; off <<= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+template <int L>
+__device__ inline bool team_any(bool v) {
+  const int base = (threadIdx.x & 63) & ~(L - 1);
+  const uint64_t mask = (L == 64) ? ~0ull : ((1ull << (L & 63)) - 1) << base;
+  return (__ballot(v) & mask) != 0ull;
+}
+
+// LDS written by some lanes of a wave and read by others of the same wave
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// order-preserving bits of a float; 0 is below every number and stands for "not to be chosen"
+__device__ inline uint32_t order_bits(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ inline float from_order_bits(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o); }
+
+// V consecutive elements from any address; those at `count` and beyond read as `fill`
+template <int V, typename T>
+__device__ inline void load_run(const T* p, int count, float fill, float (&v)[V]) {
+  if (count >= V) {
+    T raw[V];
+    __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = Elem<T>::load(raw + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < count ? Elem<T>::load(p + j) : fill;
+  }
+}
+template <int V, typename T>
+__device__ inline void store_run(T* p, int count, const float (&v)[V]) {
+  if (count >= V) {
+    T raw[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) Elem<T>::store(raw + j, v[j]);
+    __builtin_memcpy(p, raw, sizeof(raw));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < count) Elem<T>::store(p + j, v[j]);
+  }
+}
+
+struct RouteArgs {
+  const float* bias; int32_t* indices; float* weights; int32_t* counts;
+  int64_t N; int E, K, softmax, G, kept, top2, renorm; float scale;
+};
+
+// Drops the groups that do not stay from by[] (-inf).  `near`: how close two scores may lie for their order to be in doubt
+// (0: exact); returns whether one was.  tile: T E values, score: T G values of the wave's own LDS (C units).
+template <typename C, int V, int L>
+__device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_rel, C* tile, C* score) {
+  constexpr int T = 64 / L;
+  const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L;
+  const int size = A.E / A.G, G = A.G, e0 = tl * V;
+  const C low = -(C)INFINITY;
+  wave_sync();
+  if (size % V == 0) {
+    // whole lanes per group: the two largest of ever longer runs of lanes, up to the group's end, in its first lane
+    C a = low, b = low;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      b = by[j] > a ? a : (by[j] > b ? by[j] : b);
+      a = by[j] > a ? by[j] : a;
+    }
+    const int lanes = size / V, pos = tl % lanes;
+    for (int off = 1; off < lanes; off <<= 1) {
+      const C oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
+      if (pos + off < lanes) {
+        const C second = a > oa ? (oa > b ? oa : b) : (a > ob ? a : ob);
+        a = a > oa ? a : oa;
+        b = second;
+      }
+    }
+    if (pos == 0 && e0 < A.E) score[team * G + tl / lanes] = (A.top2 && b > low) ? a + b : a;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < A.E) tile[team * A.E + e0 + j] = by[j];
+    wave_sync();
+    for (int p = lane; p < T * G; p += 64) {
+      const C* q = tile + p * size;       // team-major, groups in order: p counts both
+      C a = low, b = low;
+      for (int i = 0; i < size; ++i) {
+        const C v = q[i];
+        b = v > a ? a : (v > b ? v : b);
+        a = v > a ? v : a;
+      }
+      score[p] = (A.top2 && b > low) ? a + b : a;
+    }
+  }
+  wave_sync();
+  bool doubt = false;
+  uint8_t* stays = (uint8_t*)tile;
+  for (int p = lane; p < T * G; p += 64) {
+    const C* all = score + p / G * G;
+    const int g = p % G;
+    const C mine = all[g];
+    const C size_of = mine < 0 ? -mine : mine;
+    const C near_by = (near_abs > 0 && size_of < (C)INFINITY) ? near_abs + near_rel * size_of : (C)0;
+    int ahead = 0, surely = 0, maybe = 0;
+    for (int o = 0; o < G; ++o) {
+      const C v = all[o];
+      ahead += (v > mine || (v == mine && o < g)) ? 1 : 0;
+      surely += (v > mine + near_by) ? 1 : 0;
+      maybe += (o != g && v >= mine - near_by) ? 1 : 0;
+    }
+    if (near_abs > 0 && mine > low && surely < A.kept && maybe >= A.kept) doubt = true;
+    stays[p] = ahead < A.kept ? 1 : 0;
+  }
+  wave_sync();
+  int g = e0 / size, r = e0 - g * size;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (e0 + j < A.E && !stays[team * G + g]) by[j] = low;
+    if (++r == size) { r = 0; ++g; }
+  }
+  wave_sync();
+  return __ballot(doubt) != 0ull;
+}
+
+// The choice on float64 scores, with the waves' slow way of finding a maximum: returns place tl's expert (or -1).
+template <int V, int L>
+__device__ __forceinline__ int choose_exactly(const float (&z)[V], const RouteArgs& A, bool row_bad, double* lds) {
+  const int lane = threadIdx.x & 63, tl = lane & (L - 1), e0 = tl * V;
+  const double low = -(double)INFINITY;
+  double by[V];
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < V; ++j) top = fmaxf(top, z[j]);
+  top = team_max<L>(top);
+  if (!finite(top)) top = 0.f;
+  double total = 0.0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    by[j] = A.softmax ? exp((double)z[j] - (double)top) : 1.0 / (1.0 + exp(-(double)z[j]));
+    total += by[j];
+  }
+  if (A.softmax) total = team_sum<L>(total);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (A.softmax) by[j] /= total;
+    if (A.bias != nullptr && e0 + j < A.E) by[j] += (double)A.bias[e0 + j];
+    by[j] = (z[j] == -INFINITY || row_bad) ? low : by[j] + 0.0;
+  }
+  if (A.G > 1) keep_groups<double, V, L>(by, A, 0.0, 0.0, lds, lds + 64 / L * A.E);
+  int place = -1;
+  for (int i = 0; i < A.K; ++i) {
+    double v = low;
+    int at = MAX_E;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (by[j] > v) { v = by[j]; at = e0 + j; }
+#pragma unroll
+    for (int off = 1; off < L; off <<= 1) {
+      const double ov = __shfl_xor(v, off, kWave);
+      const int oa = __shfl_xor(at, off, kWave);
+      if (ov > v || (ov == v && oa < at)) { v = ov; at = oa; }
+    }
+    if (tl == i) place = v > low ? at : -1;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e0 + j == at) by[j] = low;
+  }
+  return place;
+}
+
+// DIRECT: the choice goes by the logits themselves (an instance of its own: without the float64 choice it needs 60 registers
+// less, and the order of the scores is that of the logits, so nothing is in doubt).
+template <typename T, int V, int L, bool DIRECT>
+__global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restrict__ logits, T* __restrict__ routing, const RouteArgs A,
+                                                                int wave_lds) {
+  extern __shared__ __align__(16) char lds_raw[];
+  constexpr int TOK = 64 / L;
+  const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
+  char* lds = lds_raw + (threadIdx.x >> 6) * wave_lds;
+  int* hist = (int*)(lds_raw + WAVES * wave_lds);
+  if (A.counts != nullptr) {
+    for (int e = threadIdx.x; e < A.E; e += WAVES * 64) hist[e] = 0;
+    __syncthreads();
+  }
+  constexpr bool direct = DIRECT;
+  const int have = A.E - e0;                             // experts from e0 on (<= 0: an idle lane)
+  const int64_t tiles = (A.N + TOK - 1) / TOK;
+  for (int64_t tile = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6); tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
+    const int64_t row = tile * TOK + team;
+    const bool live = row < A.N;
+    const T* zr = logits + row * A.E;
+    float z[V];
+    load_run<V>(zr + e0, live ? have : 0, -INFINITY, z);
+    bool bad = false;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      bad = bad || z[j] != z[j] || (A.softmax && z[j] == INFINITY);
+      top = fmaxf(top, z[j]);
+    }
+    const bool whole = A.softmax && !(A.renorm && direct);      // the row's softmax is needed, not only its order
+    float sum = 1.f;
+    float p[V];
+    if (whole) {
+      top = team_max<L>(top);
+      if (!finite(top)) top = 0.f;
+      sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        p[j] = expf(z[j] - top);
+        sum += p[j];
+      }
+      sum = team_sum<L>(sum);
+    }
+    float by[V];
+    if (direct) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) by[j] = z[j] + 0.f;           // + 0: the two zeros are one value
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float c = A.softmax ? p[j] / sum : 1.f / (1.f + expf(-z[j]));
+        if (A.bias != nullptr && j < have) c += A.bias[e0 + j];
+        by[j] = z[j] == -INFINITY ? -INFINITY : c + 0.f;
+        bad = bad || by[j] != by[j];
+      }
+    }
+    bad = team_any<L>(bad);
+    if (bad) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) by[j] = -INFINITY;
+    }
+    bool doubt = false;
+    if (A.G > 1)
+      doubt = keep_groups<float, V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
+    uint64_t key[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = by[j] > -INFINITY ? ((uint64_t)order_bits(by[j]) << 32) | (uint32_t)(2 * MAX_E - (e0 + j)) : 0ull;
+    // lane's keys in descending order (odd-even merge network)
+#pragma unroll
+    for (int a = 1; a < V; a *= 2)
+#pragma unroll
+      for (int b = a; b >= 1; b /= 2)
+#pragma unroll
+        for (int j = b % a; j + b < V; j += 2 * b)
+#pragma unroll
+          for (int i = 0; i < (b < V - j - b ? b : V - j - b); ++i)
+            if ((i + j) / (2 * a) == (i + j + b) / (2 * a)) {
+              const uint64_t u = key[i + j], w = key[i + j + b];
+              key[i + j] = u > w ? u : w;
+              key[i + j + b] = u > w ? w : u;
+            }
+    uint32_t mine_hi = 0, mine_lo = 0;                          // place tl's key
+    float last = 0.f;
+    const int turns = direct ? A.K : A.K + 1;                   // one more where the runner-up may be too close
+    for (int i = 0; i < turns; ++i) {
+      const uint32_t head_hi = (uint32_t)(key[0] >> 32), head_lo = (uint32_t)key[0];
+      const uint32_t hi = team_max_u<L>(head_hi);
+      const uint32_t lo = team_max_u<L>(head_hi == hi ? head_lo : 0u);
+      if (tl == i && i < A.K) { mine_hi = hi; mine_lo = lo; }
+      if (!direct) {
+        const float c = hi != 0 ? from_order_bits(hi) : -INFINITY;
+        if (i > 0 && hi != 0 && last - c <= 0x1p-19f + 0x1p-22f * fabsf(last)) doubt = true;
+        last = c;
+      }
+      const bool won = head_lo == lo;
+#pragma unroll
+      for (int j = 0; j + 1 < V; ++j) key[j] = won ? key[j + 1] : key[j];
+      key[V - 1] = won ? 0ull : key[V - 1];
+    }
+    int at = (tl < A.K && mine_hi != 0) ? 2 * MAX_E - (int)mine_lo : -1;
+    if constexpr (!direct) {
+      if (__ballot(doubt) != 0ull) at = choose_exactly<V, L>(z, A, bad, (double*)lds);
+    }
+    // place tl's weight
+    float zi = -INFINITY;
+    if (at >= 0) zi = direct ? from_order_bits(mine_hi) : Elem<T>::load(zr + at);
+    float ref = A.softmax ? top : 0.f;
+    if (A.renorm) {
+      ref = team_max<L>(A.softmax ? zi : fminf(zi, 0.f));
+      if (!finite(ref)) ref = 0.f;
+    }
+    float w = 0.f;
+    if (at >= 0) w = A.softmax ? expf(zi - ref) : expf(fminf(zi, 0.f) - ref) / (1.f + expf(-fabsf(zi)));
+    float total = A.softmax ? sum : 1.f;
+    if (A.renorm) total = team_sum<L>(w);
+    w = at >= 0 ? A.scale * (w / total) : 0.f;
+    if (tl < A.K && live) {
+      if (A.indices) A.indices[row * A.K + tl] = at;
+      if (A.weights) A.weights[row * A.K + tl] = w;
+      if (A.counts != nullptr && at >= 0) atomicAdd(hist + at, 1);
+    }
+    if (routing) {
+      T* dense = (T*)lds;                                       // [TOK][E], as the rows lie in memory
+      const int rows = (int)((A.N - tile * TOK < TOK) ? A.N - tile * TOK : TOK);
+      const int n = rows * A.E;
+      wave_sync();
+      for (int i = lane * (16 / (int)sizeof(T)); i < TOK * A.E; i += 64 * (16 / (int)sizeof(T))) *(uint4*)(dense + i) = make_uint4(0, 0, 0, 0);
+      wave_sync();
+      if (at >= 0) Elem<T>::store(dense + team * A.E + at, w);
+      wave_sync();
+      T* out = routing + tile * TOK * A.E;
+      constexpr int C = 16 / (int)sizeof(T);
+      for (int i = lane * C; i < n; i += 64 * C) {
+        if (i + C <= n) {
+          const uint4 v = *(const uint4*)(dense + i);
+          __builtin_memcpy(out + i, &v, 16);
+        } else {
+          for (int j = i; j < n; ++j) out[j] = dense[j];
+        }
+      }
+      wave_sync();
+    }
+  }
+  if (A.counts != nullptr) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < A.E; e += WAVES * 64)
+      if (hist[e] != 0) atomicAdd(A.counts + e, hist[e]);
+  }
+}
+
+// Gradient by the same teams: lane i has place i (expert, score, gradient), the places' gradients meet in an LDS tile of the
+// wave's rows, and every lane adds the softmax's common term to its V experts where there is one.  The logits are gathered at
+// the chosen experts; whole rows of them are read only for softmax scores that are not renormalised.
+template <typename T, int V, int L>
+__global__ __launch_bounds__(WAVES * 64) void route_grad_team_kernel(const T* __restrict__ logits, const int32_t* __restrict__ indices,
+                                                                     const T* __restrict__ g_routing, const float* __restrict__ g_weights,
+                                                                     T* __restrict__ grad, int64_t N, int E, int K, int softmax, int renorm,
+                                                                     float scale) {
+  constexpr int TOK = 64 / L;
+  __shared__ __align__(16) float tiles_raw[WAVES][64 * V];
+  const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
+  float* own = tiles_raw[threadIdx.x >> 6] + team * L * V;      // this token's row (L V >= E)
+  const bool whole = softmax && !renorm;
+  const int64_t tiles = (N + TOK - 1) / TOK;
+  for (int64_t tile = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6); tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
+    const int64_t row = tile * TOK + team;
+    const bool live = row < N;
+    int at = (live && tl < K) ? indices[row * K + tl] : -1;
+    if (at >= E) at = -1;
+    float zi = -INFINITY, q = 0.f;
+    if (at >= 0) {
+      zi = Elem<T>::load(logits + row * E + at);
+      if (g_routing) q = Elem<T>::load(g_routing + row * E + at);
+      if (g_weights) q += g_weights[row * K + tl];
+    }
+    float z[V], top = 0.f, sum = 1.f;
+    if (whole) {
+      load_run<V>(logits + row * E + e0, live ? E - e0 : 0, -INFINITY, z);
+      top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < V; ++j) top = fmaxf(top, z[j]);
+      top = team_max<L>(top);
+      if (!finite(top)) top = 0.f;
+      sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        z[j] = expf(z[j] - top);
+        sum += z[j];
+      }
+      sum = team_sum<L>(sum);
+    }
+    float ref = top;
+    if (renorm) {
+      ref = team_max<L>(softmax ? zi : fminf(zi, 0.f));
+      if (!finite(ref)) ref = 0.f;
+    }
+    float s = 0.f;
+    if (at >= 0) s = softmax ? expf(zi - ref) : expf(fminf(zi, 0.f) - ref) / (1.f + expf(-fabsf(zi)));
+    if (renorm) {
+      sum = team_sum<L>(s);
+      q -= __shfl(at >= 0 ? q : 0.f, lane & ~(L - 1), kWave);   // less the first place's: no effect but on the rounding
+    }
+    const float p = at >= 0 ? s / sum : 0.f;
+    const float dot = (whole || renorm) ? team_sum<L>(at >= 0 ? p * q : 0.f) : 0.f;
+    float d = scale * p * (q - (renorm ? dot : 0.f));
+    if (!softmax) d = at >= 0 ? d / (1.f + expf(zi)) : 0.f;
+    const bool some = team_any<L>(at >= 0);
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < V; j += 4) *(float4*)(own + e0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+    wave_sync();
+    if (at >= 0) atomicAdd(own + at, d);
+    wave_sync();
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 f = *(const float4*)(own + e0 + j);
+      v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
+    }
+    if (whole && some) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] -= scale * (z[j] / sum) * dot;
+    }
+    if (live && e0 < E) store_run<V>(grad + row * E + e0, E - e0, v);
+  }
+}
+
+// More than 64 places: one wave per token, float64 throughout.
 template <typename T>
 __global__ __launch_bounds__(64) void route_kernel(const T* __restrict__ logits, const float* __restrict__ bias, T* __restrict__ routing,
                                                    int32_t* __restrict__ indices, float* __restrict__ weights,
@@ -200,6 +651,7 @@ __global__ __launch_bounds__(64) void route_kernel(const T* __restrict__ logits,
 //   renormalised: w_j (q_j - sum q_i p_i), p = w / scale, times (1 - s_j) for sigmoid scores; q less its first value, which
 //   changes nothing and keeps the difference exact where one expert has nearly all the weight
 //   softmax as it is: scale s_j (q_j [chosen] - sum q_i s_i)       sigmoid as it is: scale q_j s_j (1 - s_j)
+// (more than 64 places: one wave per token)
 template <typename T>
 __global__ __launch_bounds__(64) void route_grad_kernel(const T* __restrict__ logits, const int32_t* __restrict__ indices,
                                                         const T* __restrict__ g_routing, const float* __restrict__ g_weights,
@@ -265,19 +717,81 @@ __global__ __launch_bounds__(64) void route_grad_kernel(const T* __restrict__ lo
   }
 }
 
+// Lanes per token: as many as the places and, at V experts per lane, the experts need.
+inline int team_lanes(int E, int V, int K) {
+  int lanes = 4;
+  while (lanes * V < E || lanes < K) lanes *= 2;
+  return lanes;
+}
+
+inline unsigned team_grid(int64_t N, int L) {
+  const int64_t blocks = cdiv64(cdiv64(N, 64 / L), WAVES);
+  return (unsigned)(blocks < 4096 ? blocks : 4096);
+}
+
+template <typename T, int V, int L>
+hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, const RouteArgs& A, hipStream_t s) {
+  // per wave: the dense tile, and with groups the choices and the groups' scores in float64 (the exact choice's)
+  size_t wave = (size_t)(64 / L) * A.E * sizeof(T);
+  if (A.G > 1) wave = (size_t)(64 / L) * (A.E + A.G) * sizeof(double);
+  wave = (wave + 15) / 16 * 16;
+  const size_t lds = WAVES * wave + (A.counts ? (size_t)A.E * 4 : 0);
+  const bool direct = A.bias == nullptr && !(A.G > 1 && A.top2);
+  const auto kern = direct ? route_team_kernel<T, V, L, true> : route_team_kernel<T, V, L, false>;
+  if (lds > (64u << 10)) {   // (E > 512 with hundreds of groups)
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(kern, dim3(team_grid(sh.n_tokens, L)), dim3(WAVES * 64), lds, s, logits, routing, A, (int)wave);
+  return hipGetLastError();
+}
+
 template <typename T>
 hipError_t forward_t(const d2dmoe_route_shape& sh, const void* logits, const float* bias, void* routing, int32_t* indices, float* weights,
                      int32_t* counts, hipStream_t s) {
+  const int softmax = sh.scoring == D2DMOE_SCORE_SOFTMAX, top2 = sh.group_score == D2DMOE_GROUP_TOP2;
+  if (sh.k <= 64) {
+    const RouteArgs A{bias, indices, weights, counts, sh.n_tokens, sh.n_experts, sh.k, softmax, sh.n_groups, sh.kept_groups, top2,
+                      sh.renormalise, sh.scale};
+    const T* z = (const T*)logits;
+    T* r = (T*)routing;
+    if (sh.n_experts > 512) return forward_l<T, 16, 64>(sh, z, r, A, s);
+    switch (team_lanes(sh.n_experts, 8, sh.k)) {
+      case 4: return forward_l<T, 8, 4>(sh, z, r, A, s);
+      case 8: return forward_l<T, 8, 8>(sh, z, r, A, s);
+      case 16: return forward_l<T, 8, 16>(sh, z, r, A, s);
+      case 32: return forward_l<T, 8, 32>(sh, z, r, A, s);
+      default: return forward_l<T, 8, 64>(sh, z, r, A, s);
+    }
+  }
   const unsigned grid = (unsigned)(sh.n_tokens < (1 << 20) ? sh.n_tokens : (1 << 20));
   hipLaunchKernelGGL(route_kernel<T>, dim3(grid), dim3(64), 0, s, (const T*)logits, bias, (T*)routing, indices, weights, counts,
-                     sh.n_tokens, sh.n_experts, sh.k, sh.scoring == D2DMOE_SCORE_SOFTMAX, sh.n_groups, sh.kept_groups,
-                     sh.group_score == D2DMOE_GROUP_TOP2, sh.renormalise, sh.scale);
+                     sh.n_tokens, sh.n_experts, sh.k, softmax, sh.n_groups, sh.kept_groups, top2, sh.renormalise, sh.scale);
+  return hipGetLastError();
+}
+
+template <typename T, int V, int L>
+hipError_t backward_l(const d2dmoe_route_shape& sh, const void* logits, const int32_t* indices, const void* g_routing,
+                      const float* g_weights, void* grad, hipStream_t s) {
+  hipLaunchKernelGGL((route_grad_team_kernel<T, V, L>), dim3(team_grid(sh.n_tokens, L)), dim3(WAVES * 64), 0, s, (const T*)logits, indices,
+                     (const T*)g_routing, g_weights, (T*)grad, sh.n_tokens, sh.n_experts, sh.k, sh.scoring == D2DMOE_SCORE_SOFTMAX,
+                     sh.renormalise, sh.scale);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t backward_t(const d2dmoe_route_shape& sh, const void* logits, const int32_t* indices, const void* g_routing,
                       const float* g_weights, void* grad, hipStream_t s) {
+  if (sh.k <= 64) {
+    if (sh.n_experts > 512) return backward_l<T, 16, 64>(sh, logits, indices, g_routing, g_weights, grad, s);
+    switch (team_lanes(sh.n_experts, 8, sh.k)) {
+      case 4: return backward_l<T, 8, 4>(sh, logits, indices, g_routing, g_weights, grad, s);
+      case 8: return backward_l<T, 8, 8>(sh, logits, indices, g_routing, g_weights, grad, s);
+      case 16: return backward_l<T, 8, 16>(sh, logits, indices, g_routing, g_weights, grad, s);
+      case 32: return backward_l<T, 8, 32>(sh, logits, indices, g_routing, g_weights, grad, s);
+      default: return backward_l<T, 8, 64>(sh, logits, indices, g_routing, g_weights, grad, s);
+    }
+  }
   const unsigned grid = (unsigned)(sh.n_tokens < (1 << 20) ? sh.n_tokens : (1 << 20));
   hipLaunchKernelGGL(route_grad_kernel<T>, dim3(grid), dim3(64), 0, s, (const T*)logits, indices, (const T*)g_routing, g_weights,
                      (T*)grad, sh.n_tokens, sh.n_experts, sh.k, sh.scoring == D2DMOE_SCORE_SOFTMAX, sh.renormalise, sh.scale);
