@@ -6,8 +6,12 @@
 //
 // All sums, the statistics and every intermediate are float32; what is stored in 16 bits is rounded once (h = x + residual
 // is such a value: it is the residual stream, an output, and the norm is taken of what the stream holds).
-#include "common.hpp"
+//
+// Two kernels per direction: one that keeps a row in registers (any width up to 16384), one that passes over it again for
+// every use (wider rows, and rows narrower than one vector).
 #include "launch.hpp"
+#include "mfma_common.hpp"
+#include "team.hpp"
 
 namespace d2dmoe {
 
@@ -15,6 +19,305 @@ namespace {
 
 constexpr int NT = 256;   // threads per workgroup
 
+// ---------------------------------------------------------------------------------------------------------------------
+// A row in registers.  TPR threads per row: one wave (four rows per workgroup, no barrier) or a whole workgroup, CH vectors
+// of 16 bytes each.  All but the last of the CH are whole; in the last one a thread may lie behind the row's end (it reads
+// the row's first vector and drops it) or across it (it reads the row's last whole vector, of which it counts the elements
+// nobody else has; the others are computed twice and stored twice, with the same bits).  Rows may begin at any element: the
+// loads and stores make no claim on alignment.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
+
+template <typename T> __device__ __forceinline__ void decode(const uint4& raw, float (&v)[kVec<T>]) {
+  const uint32_t q[4] = {raw.x, raw.y, raw.z, raw.w};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(q[i]);
+  } else {
+    constexpr bool F16 = Elem<T>::dtype == D2DMOE_F16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = dec16<F16>(q[i] & 0xffffu);
+      v[2 * i + 1] = dec16_hi<F16>(q[i]);
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 encode(const float (&v)[kVec<T>]) {
+  uint32_t q[4];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = enc16x2<Elem<T>::dtype == D2DMOE_F16>(v[2 * i], v[2 * i + 1]);
+  }
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+template <typename T> __device__ __forceinline__ uint4 load16(const T* p) {
+  uint4 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void store16(T* p, const uint4& r) { __builtin_memcpy(p, &r, 16); }
+
+// V parameters as float32
+template <typename P, int V> __device__ __forceinline__ void load_params(const P* p, float (&v)[V]) {
+  P raw[V];
+  __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = Elem<P>::load(raw + j);
+}
+
+// Sums of two values over the TPR threads of a row.  `turn` alternates between calls: the next call writes the other half of
+// buf, and the one after comes behind a barrier that every reader of this half has passed, so one barrier each is enough.
+template <int TPR>
+__device__ __forceinline__ void row_sum(float& a, float& b, float (*buf)[2][TPR / 64], int& turn) {
+  a = team_sum<64>(a);
+  b = team_sum<64>(b);
+  if constexpr (TPR > 64) {
+    float (*half)[TPR / 64] = buf[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+      half[0][threadIdx.x >> 6] = a;
+      half[1][threadIdx.x >> 6] = b;
+    }
+    lds_barrier();
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) {
+      a += half[0][i];
+      b += half[1][i];
+    }
+  }
+}
+
+struct NormForward {
+  const void *x, *residual, *weight, *bias;
+  void *sum, *out;
+  float *mean, *rstd;
+  int64_t N;
+  int D;
+  float eps;
+};
+
+template <typename T, typename P, int TPR, int CH, bool RES>
+__global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_kernel(const NormForward A) {
+  constexpr int V = kVec<T>, ROWS = TPR < NT ? NT / TPR : 1;
+  __shared__ float buf[2][2][TPR / 64];
+  int turn = 0;
+  const int t = threadIdx.x % TPR;
+  const int D = A.D;
+  int at[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) at[c] = (c * TPR + t) * V;
+  const int over = at[CH - 1] + V - D;                      // elements of the last vector behind the row's end
+  const int skip = over <= 0 ? 0 : (over >= V ? V : over);  // ... which its first `skip` elements stand for
+  if (skip == V) at[CH - 1] = 0;
+  else if (skip > 0) at[CH - 1] = D - V;
+  float w[CH][V], b[CH][V];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) { w[c][j] = 1.f; b[c][j] = 0.f; }
+    if (A.weight) load_params<P, V>((const P*)A.weight + at[c], w[c]);
+    if (A.bias) load_params<P, V>((const P*)A.bias + at[c], b[c]);
+  }
+  const float inv_d = 1.f / (float)D;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  uint4 xr[CH], rr[CH];
+  auto request = [&](int64_t r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      xr[c] = load16((const T*)A.x + r * D + at[c]);
+      if (RES) rr[c] = load16((const T*)A.residual + r * D + at[c]);
+    }
+  };
+  if (row < A.N) request(row);
+  for (; row < A.N; row += step) {
+    float h[CH][V];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      decode<T>(xr[c], h[c]);
+      if (RES) {
+        float r[V];
+        decode<T>(rr[c], r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[c][j] += r[j];
+        const uint4 packed = encode<T>(h[c]);               // the stream as it is stored is what the norm sees
+        decode<T>(packed, h[c]);
+        if (A.sum && (c < CH - 1 || skip < V)) store16((T*)A.sum + row * D + at[c], packed);
+      }
+    }
+    if (row + step < A.N) request(row + step);              // the next row travels while this one is worked on
+    float s = 0.f, none = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += (c < CH - 1 || j >= skip) ? h[c][j] : 0.f;
+    row_sum<TPR>(s, none, buf, turn);
+    const float m = s * inv_d;
+    // the mean's own rounding error, from the centred values: it matters where the mean is far larger than the spread
+    float e = 0.f, q = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        h[c][j] -= m;
+        const float v = (c < CH - 1 || j >= skip) ? h[c][j] : 0.f;
+        e += v;
+        q = fmaf(v, v, q);
+      }
+    row_sum<TPR>(e, q, buf, turn);
+    const float dm = e * inv_d;
+    const float r = 1.f / sqrtf(fmaxf(q * inv_d - dm * dm, 0.f) + A.eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[c][j] = fmaf((h[c][j] - dm) * r, w[c][j], b[c][j]);
+      if (c < CH - 1 || skip < V) store16((T*)A.out + row * D + at[c], encode<T>(h[c]));
+    }
+    if (t == 0) {
+      if (A.mean) A.mean[row] = m + dm;
+      if (A.rstd) A.rstd[row] = r;
+    }
+  }
+}
+
+struct NormBackward {
+  const void *g, *gs, *h, *weight;
+  const float *mean, *rstd;
+  void* grad;
+  float* partial;   // [workgroup][2][D]: column sums of the workgroup's rows, or NULL
+  int64_t N;
+  int D;
+};
+
+template <typename T, typename P, int TPR, int CH>
+__global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_grad_kernel(const NormBackward A) {
+  constexpr int V = kVec<T>, ROWS = TPR < NT ? NT / TPR : 1;
+  __shared__ float buf[2][2][TPR / 64];
+  __shared__ float columns[ROWS > 1 ? 2 * TPR * CH * V : 1];
+  int turn = 0;
+  const int t = threadIdx.x % TPR;
+  const int D = A.D;
+  int at[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) at[c] = (c * TPR + t) * V;
+  const int over = at[CH - 1] + V - D;
+  const int skip = over <= 0 ? 0 : (over >= V ? V : over);
+  if (skip == V) at[CH - 1] = 0;
+  else if (skip > 0) at[CH - 1] = D - V;
+  float w[CH][V], sw[CH][V], sb[CH][V];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) { w[c][j] = 1.f; sw[c][j] = 0.f; sb[c][j] = 0.f; }
+    if (A.weight) load_params<P, V>((const P*)A.weight + at[c], w[c]);
+  }
+  const float inv_d = 1.f / (float)D;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row < A.N; row += step) {
+    uint4 gr[CH], hr[CH], sr[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      gr[c] = load16((const T*)A.g + row * D + at[c]);
+      hr[c] = load16((const T*)A.h + row * D + at[c]);
+      if (A.gs) sr[c] = load16((const T*)A.gs + row * D + at[c]);
+    }
+    const float m = A.mean[row], r = A.rstd[row];
+    float g[CH][V], n[CH][V];
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      decode<T>(gr[c], g[c]);
+      decode<T>(hr[c], n[c]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        n[c][j] = (n[c][j] - m) * r;
+        sw[c][j] = fmaf(g[c][j], n[c][j], sw[c][j]);
+        sb[c][j] += g[c][j];
+        g[c][j] *= w[c][j];
+        const float u = (c < CH - 1 || j >= skip) ? g[c][j] : 0.f;
+        a += u;
+        b = (c < CH - 1 || j >= skip) ? fmaf(u, n[c][j], b) : b;
+      }
+    }
+    row_sum<TPR>(a, b, buf, turn);
+    a *= inv_d;
+    b *= inv_d;
+    if (A.grad) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        float s[V];
+        if (A.gs) decode<T>(sr[c], s);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float v = r * (g[c][j] - a - n[c][j] * b);
+          g[c][j] = A.gs ? v + s[j] : v;
+        }
+        if (c < CH - 1 || skip < V) store16((T*)A.grad + row * D + at[c], encode<T>(g[c]));
+      }
+    }
+  }
+  if (A.partial == nullptr) return;
+  float* out = A.partial + (int64_t)blockIdx.x * 2 * D;
+  if constexpr (ROWS == 1) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c < CH - 1 || j >= skip) {
+          out[at[c] + j] = sw[c][j];
+          out[D + at[c] + j] = sb[c][j];
+        }
+  } else {
+    // the waves' sums one after the other, in wave order
+    for (int i = 0; i < ROWS; ++i) {
+      if ((int)threadIdx.x / TPR == i) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (c < CH - 1 || j >= skip) {
+              float* p = columns + at[c] + j;
+              p[0] = i == 0 ? sw[c][j] : p[0] + sw[c][j];
+              p[D] = i == 0 ? sb[c][j] : p[D] + sb[c][j];
+            }
+      }
+      __syncthreads();
+    }
+    for (int d = threadIdx.x; d < 2 * D; d += NT) out[d] = columns[d];
+  }
+}
+
+// The workgroups' column sums added in a fixed order.  Workgroup = 32 of the 2 D columns, 32 threads per column: thread q adds
+// the workgroups q, q + 32, ...; then the 32 in order.
+template <typename P>
+__global__ __launch_bounds__(1024) void layer_norm_grad_finish_kernel(const float* __restrict__ partial, P* __restrict__ gw,
+                                                                      P* __restrict__ gb, int parts, int D) {
+  __shared__ float part[32][33];
+  const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int d = (int)blockIdx.x * 32 + c;
+  float s = 0.f;
+  if (d < 2 * D) {
+#pragma unroll 4
+    for (int i = q; i < parts; i += 32) s += partial[(int64_t)i * 2 * D + d];
+  }
+  part[q][c] = s;
+  __syncthreads();
+  if (threadIdx.x < 32 && d < 2 * D) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v += part[i][c];
+    P* out = d < D ? gw : gb;
+    if (out != nullptr) Elem<P>::store(out + (d < D ? d : d - D), v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Any width: one workgroup per row, a pass over it for every use.
+// ---------------------------------------------------------------------------------------------------------------------
 __device__ inline float wave_sum(float v) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
@@ -125,24 +428,68 @@ __global__ __launch_bounds__(NT) void layer_norm_grad_columns_kernel(const T* __
   }
 }
 
-// The slabs' column sums added in order: thread = column of grad_weight (blockIdx.y == 0) or grad_bias.
-template <typename P>
-__global__ __launch_bounds__(NT) void layer_norm_grad_finish_kernel(const float* __restrict__ partial, P* __restrict__ gw,
-                                                                    P* __restrict__ gb, int slabs, int D) {
-  const int d = (int)blockIdx.x * NT + threadIdx.x;
-  P* out = blockIdx.y ? gb : gw;
-  if (d >= D || out == nullptr) return;
-  const float* p = partial + (blockIdx.y ? D : 0) + d;
-  float s = 0.f;
-  for (int i = 0; i < slabs; ++i) s += p[(int64_t)i * 2 * D];
-  Elem<P>::store(out + d, s);
+inline int slab_count(int64_t N) { return (int)(N < 64 ? 1 : (cdiv64(N, 64) < 256 ? cdiv64(N, 64) : 256)); }
+
+// Threads per row and vectors per thread for a width, or TPR = 0 where the row does not fit.  Up to four vectors per thread
+// (32 16-bit values, with the column sums 160 registers); a wave per row as long as that is enough, then a workgroup.
+struct RowPlan { int tpr, ch; };
+template <typename T> RowPlan row_plan(int D) {
+  constexpr int V = kVec<T>;
+  if (D < V) return {0, 0};
+  const int vectors = (D + V - 1) / V;
+  if (vectors <= 64 * 4) return {64, (vectors + 63) / 64};
+  if (vectors <= 256 * 4) return {256, (vectors + 255) / 256};
+  if (vectors <= 1024 * 2) return {1024, 2};
+  return {0, 0};
 }
 
-inline int slab_count(int64_t N) { return (int)(N < 64 ? 1 : (cdiv64(N, 64) < 256 ? cdiv64(N, 64) : 256)); }
+// Workgroups of the row kernels: enough to fill the machine's 256 CUs, each with as many rows as that leaves it.  (A constant:
+// the workspace and the order of the column sums depend on it.)
+inline unsigned row_grid(int64_t N, int rows, int per_cu) {
+  const int64_t need = cdiv64(N, rows), most = (int64_t)256 * per_cu;
+  return (unsigned)(need < most ? need : most);
+}
+inline int grad_parts(const d2dmoe_norm_shape& sh, int tpr) { return (int)row_grid(sh.n_rows, tpr < NT ? NT / tpr : 1, tpr == 1024 ? 1 : 2); }
+
+template <typename T, typename P, int TPR, int CH>
+hipError_t forward_rows(const NormForward& A, hipStream_t s) {
+  constexpr int threads = TPR < NT ? NT : TPR;
+  const unsigned grid = row_grid(A.N, TPR < NT ? NT / TPR : 1, TPR == 1024 ? 2 : 5);
+  if (A.residual) hipLaunchKernelGGL((layer_norm_kernel<T, P, TPR, CH, true>), dim3(grid), dim3(threads), 0, s, A);
+  else hipLaunchKernelGGL((layer_norm_kernel<T, P, TPR, CH, false>), dim3(grid), dim3(threads), 0, s, A);
+  return hipGetLastError();
+}
+
+template <typename T, typename P, int TPR, int CH>
+hipError_t backward_rows(const NormBackward& A, unsigned grid, hipStream_t s) {
+  hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, TPR, CH>), dim3(grid), dim3(TPR < NT ? NT : TPR), 0, s, A);
+  return hipGetLastError();
+}
+
+#define D2DMOE_ROW_DISPATCH(PLAN, CALL)             \
+  switch (PLAN.tpr * 8 + PLAN.ch) {                 \
+    case 64 * 8 + 1: e = CALL(64, 1); break;        \
+    case 64 * 8 + 2: e = CALL(64, 2); break;        \
+    case 64 * 8 + 3: e = CALL(64, 3); break;        \
+    case 64 * 8 + 4: e = CALL(64, 4); break;        \
+    case 256 * 8 + 2: e = CALL(256, 2); break;      \
+    case 256 * 8 + 3: e = CALL(256, 3); break;      \
+    case 256 * 8 + 4: e = CALL(256, 4); break;      \
+    default: e = CALL(1024, 2); break;              \
+  }
 
 template <typename T, typename P>
 hipError_t forward_t(const d2dmoe_norm_shape& sh, const void* x, const void* residual, const void* weight, const void* bias, void* sum,
                      void* out, float* mean, float* rstd, hipStream_t s) {
+  const RowPlan plan = row_plan<T>(sh.width);
+  hipError_t e;
+  if (plan.tpr != 0) {
+    const NormForward A{x, residual, weight, bias, sum, out, mean, rstd, sh.n_rows, sh.width, sh.eps};
+#define D2DMOE_ROWS(TPR, CH) forward_rows<T, P, TPR, CH>(A, s)
+    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS)
+#undef D2DMOE_ROWS
+    return e;
+  }
   const unsigned grid = (unsigned)(sh.n_rows < 65536 ? sh.n_rows : 65536);
   hipLaunchKernelGGL((layer_norm_rows_kernel<T, P>), dim3(grid), dim3(NT), 0, s, (const T*)x, (const T*)residual, (const P*)weight,
                      (const P*)bias, (T*)sum, (T*)out, mean, rstd, sh.n_rows, sh.width, sh.eps);
@@ -154,30 +501,43 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
                       const float* rstd, void* grad, void* gw, void* gb, void* workspace, hipStream_t s) {
   const int64_t N = sh.n_rows;
   const int D = sh.width;
-  if (N > 0 && grad != nullptr) {
-    const unsigned grid = (unsigned)(N < 65536 ? N : 65536);
-    hipLaunchKernelGGL((layer_norm_grad_rows_kernel<T, P>), dim3(grid), dim3(NT), 0, s, (const T*)g, (const T*)gs, (const T*)h,
-                       (const P*)weight, mean, rstd, (T*)grad, N, D);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+  const bool columns = gw != nullptr || gb != nullptr;
+  int parts = 0;                       // partial column sums in the workspace
+  hipError_t e = hipSuccess;
+  const RowPlan plan = row_plan<T>(D);
+  if (N > 0 && plan.tpr != 0) {
+    parts = grad_parts(sh, plan.tpr);
+    const NormBackward A{g, gs, h, weight, mean, rstd, grad, columns ? (float*)workspace : nullptr, N, D};
+#define D2DMOE_ROWS(TPR, CH) backward_rows<T, P, TPR, CH>(A, (unsigned)parts, s)
+    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS)
+#undef D2DMOE_ROWS
+  } else if (N > 0) {
+    if (grad != nullptr) {
+      const unsigned grid = (unsigned)(N < 65536 ? N : 65536);
+      hipLaunchKernelGGL((layer_norm_grad_rows_kernel<T, P>), dim3(grid), dim3(NT), 0, s, (const T*)g, (const T*)gs, (const T*)h,
+                         (const P*)weight, mean, rstd, (T*)grad, N, D);
+      e = hipGetLastError();
+    }
+    if (e == hipSuccess && columns) {
+      parts = slab_count(N);
+      hipLaunchKernelGGL((layer_norm_grad_columns_kernel<T>), dim3((unsigned)((D + 63) / 64), (unsigned)parts), dim3(NT), 0, s,
+                         (const T*)g, (const T*)h, mean, rstd, (float*)workspace, N, D, cdiv64(N, parts));
+      e = hipGetLastError();
+    }
   }
-  if (gw == nullptr && gb == nullptr) return hipSuccess;
-  const int slabs = N > 0 ? slab_count(N) : 0;
-  if (slabs > 0) {
-    hipLaunchKernelGGL((layer_norm_grad_columns_kernel<T>), dim3((unsigned)((D + 63) / 64), (unsigned)slabs), dim3(NT), 0, s,
-                       (const T*)g, (const T*)h, mean, rstd, (float*)workspace, N, D, cdiv64(N, slabs));
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL((layer_norm_grad_finish_kernel<P>), dim3((unsigned)((D + NT - 1) / NT), 2), dim3(NT), 0, s,
-                     (const float*)workspace, (P*)gw, (P*)gb, slabs, D);
+  if (e != hipSuccess || !columns) return e;
+  hipLaunchKernelGGL((layer_norm_grad_finish_kernel<P>), dim3((unsigned)((2 * D + 31) / 32)), dim3(1024), 0, s,
+                     (const float*)workspace, (P*)gw, (P*)gb, parts, D);
   return hipGetLastError();
 }
 
 }  // namespace
 
 size_t layer_norm_workspace_bytes(const d2dmoe_norm_shape& sh) {
-  return sh.n_rows > 0 ? (size_t)slab_count(sh.n_rows) * 2 * sh.width * sizeof(float) : 0;
+  if (sh.n_rows <= 0) return 0;
+  const RowPlan plan = sh.dtype == D2DMOE_F32 ? row_plan<float>(sh.width) : row_plan<bf16_t>(sh.width);
+  const int parts = plan.tpr != 0 ? grad_parts(sh, plan.tpr) : slab_count(sh.n_rows);
+  return (size_t)parts * 2 * sh.width * sizeof(float);
 }
 
 // (activations, parameters): both of one type, or 16-bit activations with float32 parameters

@@ -11,6 +11,7 @@
 // rows, and indices are whole numbers.  The weights are float32.
 #include "common.hpp"
 #include "launch.hpp"
+#include "team.hpp"
 
 namespace d2dmoe {
 
@@ -51,49 +52,6 @@ __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 // one that goes -- the wave repeats its choice on float64 scores; a row or two in a thousand do.
 // =====================================================================================================
 constexpr int WAVES = 4;   // per workgroup
-
-template <int CTRL>
-__device__ inline uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
-
-// All-reduce over aligned teams of L lanes: neighbours, pairs, quads (mirror of 8), eights (mirror of 16), rows, halves.
-template <int L, typename Op>
-__device__ inline uint32_t team_reduce(uint32_t v, Op op) {
-  if constexpr (L >= 2) v = op(v, dpp<0xB1>(v));
-  if constexpr (L >= 4) v = op(v, dpp<0x4E>(v));
-  if constexpr (L >= 8) v = op(v, dpp<0x141>(v));
-  if constexpr (L >= 16) v = op(v, dpp<0x140>(v));
-  if constexpr (L >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = op(r[0], r[1]);
-  }
-  if constexpr (L >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = op(r[0], r[1]);
-  }
-  return v;
-}
-template <int L>
-__device__ inline uint32_t team_max_u(uint32_t v) { return team_reduce<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
-template <int L>
-__device__ inline float team_max(float v) {
-  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
-}
-template <int L>
-__device__ inline float team_sum(float v) {
-  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
-}
-template <int L>
-__device__ inline double team_sum(double v) {
-#pragma unroll
-  for (int off = 1; off < L; off <<= 1) v += __shfl_xor(v, off, kWave);
-  return v;
-}
-template <int L>
-__device__ inline bool team_any(bool v) {
-  const int base = (threadIdx.x & 63) & ~(L - 1);
-  const uint64_t mask = (L == 64) ? ~0ull : ((1ull << (L & 63)) - 1) << base;
-  return (__ballot(v) & mask) != 0ull;
-}
 
 // LDS written by some lanes of a wave and read by others of the same wave
 __device__ inline void wave_sync() {
