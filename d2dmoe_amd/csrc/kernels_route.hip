@@ -66,6 +66,85 @@ __device__ inline uint32_t order_bits(float v) {
 }
 __device__ inline float from_order_bits(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o); }
 
+// A lane's V choices as keys that compare as unsigned numbers, the larger choice first and the lower index first among equal
+// ones: 64 bits (order of a float32, index), or 32 where the choice is a 16-bit logit.
+template <typename T, int V, bool WIDE> struct Keys {
+  uint32_t hi[V], lo[V];   // narrow: lo alone
+  __device__ __forceinline__ void set(int j, float c, int e) {
+    const uint32_t low = (uint32_t)(2 * MAX_E - e);
+    if constexpr (WIDE) {
+      hi[j] = c > -INFINITY ? order_bits(c) : 0u;
+      lo[j] = c > -INFINITY ? low : 0u;
+    } else {
+      T raw;
+      Elem<T>::store(&raw, c);
+      uint16_t u;
+      __builtin_memcpy(&u, &raw, 2);
+      const uint32_t o = (u & 0x8000u) ? (~(uint32_t)u & 0xffffu) : (u | 0x8000u);
+      lo[j] = c > -INFINITY ? (o << 16 | low) : 0u;
+    }
+  }
+  __device__ __forceinline__ void order(int i, int k) {   // larger key to place i
+    const uint32_t al = lo[i], bl = lo[k];
+    if constexpr (WIDE) {
+      const uint32_t ah = hi[i], bh = hi[k];
+      const bool swap = ((uint64_t)bh << 32 | bl) > ((uint64_t)ah << 32 | al);
+      const uint32_t ch = swap ? bh : ah, dh = swap ? ah : bh, cl = swap ? bl : al, dl = swap ? al : bl;
+      hi[i] = ch; hi[k] = dh; lo[i] = cl; lo[k] = dl;
+    } else {
+      const uint32_t big = al > bl ? al : bl, small = al > bl ? bl : al;
+      lo[i] = big; lo[k] = small;
+    }
+  }
+  __device__ __forceinline__ void sort() {   // descending (odd-even merge network)
+#pragma unroll
+    for (int a = 1; a < V; a *= 2)
+#pragma unroll
+      for (int b = a; b >= 1; b /= 2)
+#pragma unroll
+        for (int j = b % a; j + b < V; j += 2 * b)
+#pragma unroll
+          for (int i = 0; i < (b < V - j - b ? b : V - j - b); ++i)
+            if ((i + j) / (2 * a) == (i + j + b) / (2 * a)) order(i + j, i + j + b);
+  }
+  // the team's largest key, which leaves its lane's list
+  template <int L> __device__ __forceinline__ void take(uint32_t& h, uint32_t& l) {
+    if constexpr (WIDE) {
+      h = team_max_u<L>(hi[0]);
+      l = team_max_u<L>(hi[0] == h ? lo[0] : 0u);
+    } else {
+      h = l = team_max_u<L>(lo[0]);
+    }
+    const bool won = lo[0] == l;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {      // (values, not places, to choose from: the lists stay in registers)
+      const uint32_t lc = lo[j], ln = j + 1 < V ? lo[j + 1 < V ? j + 1 : j] : 0u;
+      lo[j] = won ? ln : lc;
+      if constexpr (WIDE) {
+        const uint32_t hc = hi[j], hn = j + 1 < V ? hi[j + 1 < V ? j + 1 : j] : 0u;
+        hi[j] = won ? hn : hc;
+      }
+    }
+  }
+  static __device__ __forceinline__ int expert(uint32_t l) { return 2 * MAX_E - (int)(WIDE ? l : (l & 0xffffu)); }
+  static __device__ __forceinline__ float choice(uint32_t h) {
+    if constexpr (WIDE) {
+      return from_order_bits(h);
+    } else {
+      const uint32_t o = h >> 16;
+      const uint16_t u = (uint16_t)((o & 0x8000u) ? (o ^ 0x8000u) : ~o);
+      T raw;
+      __builtin_memcpy(&raw, &u, 2);
+      return Elem<T>::load(&raw);
+    }
+  }
+};
+
+__device__ inline float larger(float a, float b) { return fmaxf(a, b); }
+__device__ inline double larger(double a, double b) { return fmax(a, b); }
+__device__ inline float smaller(float a, float b) { return fminf(a, b); }
+__device__ inline double smaller(double a, double b) { return fmin(a, b); }
+
 // V consecutive elements from any address; those at `count` and beyond read as `fill`
 template <int V, typename T>
 __device__ inline void load_run(const T* p, int count, float fill, float (&v)[V]) {
@@ -112,16 +191,15 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
     C a = low, b = low;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      b = by[j] > a ? a : (by[j] > b ? by[j] : b);
-      a = by[j] > a ? by[j] : a;
+      b = larger(b, smaller(a, by[j]));
+      a = larger(a, by[j]);
     }
     const int lanes = size / V, pos = tl % lanes;
     for (int off = 1; off < lanes; off <<= 1) {
       const C oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
       if (pos + off < lanes) {
-        const C second = a > oa ? (oa > b ? oa : b) : (a > ob ? a : ob);
-        a = a > oa ? a : oa;
-        b = second;
+        b = larger(larger(b, ob), smaller(a, oa));
+        a = larger(a, oa);
       }
     }
     if (pos == 0 && e0 < A.E) score[team * G + tl / lanes] = (A.top2 && b > low) ? a + b : a;
@@ -135,8 +213,8 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
       C a = low, b = low;
       for (int i = 0; i < size; ++i) {
         const C v = q[i];
-        b = v > a ? a : (v > b ? v : b);
-        a = v > a ? v : a;
+        b = larger(b, smaller(a, v));
+        a = larger(a, v);
       }
       score[p] = (A.top2 && b > low) ? a + b : a;
     }
@@ -282,48 +360,31 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     bool doubt = false;
     if (A.G > 1)
       doubt = keep_groups<float, V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
-    uint64_t key[V];
+    using K = Keys<T, V, !DIRECT || sizeof(T) == 4>;
+    K keys;
 #pragma unroll
-    for (int j = 0; j < V; ++j) key[j] = by[j] > -INFINITY ? ((uint64_t)order_bits(by[j]) << 32) | (uint32_t)(2 * MAX_E - (e0 + j)) : 0ull;
-    // lane's keys in descending order (odd-even merge network)
-#pragma unroll
-    for (int a = 1; a < V; a *= 2)
-#pragma unroll
-      for (int b = a; b >= 1; b /= 2)
-#pragma unroll
-        for (int j = b % a; j + b < V; j += 2 * b)
-#pragma unroll
-          for (int i = 0; i < (b < V - j - b ? b : V - j - b); ++i)
-            if ((i + j) / (2 * a) == (i + j + b) / (2 * a)) {
-              const uint64_t u = key[i + j], w = key[i + j + b];
-              key[i + j] = u > w ? u : w;
-              key[i + j + b] = u > w ? w : u;
-            }
+    for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
+    keys.sort();
     uint32_t mine_hi = 0, mine_lo = 0;                          // place tl's key
     float last = 0.f;
     const int turns = direct ? A.K : A.K + 1;                   // one more where the runner-up may be too close
     for (int i = 0; i < turns; ++i) {
-      const uint32_t head_hi = (uint32_t)(key[0] >> 32), head_lo = (uint32_t)key[0];
-      const uint32_t hi = team_max_u<L>(head_hi);
-      const uint32_t lo = team_max_u<L>(head_hi == hi ? head_lo : 0u);
-      if (tl == i && i < A.K) { mine_hi = hi; mine_lo = lo; }
+      uint32_t hi, lo;
+      keys.template take<L>(hi, lo);
+      if (tl == i) { mine_hi = hi; mine_lo = lo; }
       if (!direct) {
-        const float c = hi != 0 ? from_order_bits(hi) : -INFINITY;
+        const float c = hi != 0 ? K::choice(hi) : -INFINITY;
         if (i > 0 && hi != 0 && last - c <= 0x1p-19f + 0x1p-22f * fabsf(last)) doubt = true;
         last = c;
       }
-      const bool won = head_lo == lo;
-#pragma unroll
-      for (int j = 0; j + 1 < V; ++j) key[j] = won ? key[j + 1] : key[j];
-      key[V - 1] = won ? 0ull : key[V - 1];
     }
-    int at = (tl < A.K && mine_hi != 0) ? 2 * MAX_E - (int)mine_lo : -1;
+    int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
     if constexpr (!direct) {
       if (__ballot(doubt) != 0ull) at = choose_exactly<V, L>(z, A, bad, (double*)lds);
     }
     // place tl's weight
     float zi = -INFINITY;
-    if (at >= 0) zi = direct ? from_order_bits(mine_hi) : Elem<T>::load(zr + at);
+    if (at >= 0) zi = direct ? K::choice(mine_hi) : Elem<T>::load(zr + at);
     float ref = A.softmax ? top : 0.f;
     if (A.renorm) {
       ref = team_max<L>(A.softmax ? zi : fminf(zi, 0.f));
