@@ -35,6 +35,9 @@ __device__ inline float wave_max(float v) {
   for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
   return v;
 }
+// exp as one multiplication and the hardware's 2^x: relative error (1.5 |v| + 2) u.  For sums over a row and for choices; what
+// is stored as a weight goes through expf.
+__device__ inline float quick_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
 __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 
 // =====================================================================================================
@@ -76,12 +79,11 @@ template <typename T, int V, bool WIDE> struct Keys {
       hi[j] = c > -INFINITY ? order_bits(c) : 0u;
       lo[j] = c > -INFINITY ? low : 0u;
     } else {
-      T raw;
-      Elem<T>::store(&raw, c);
-      uint16_t u;
-      __builtin_memcpy(&u, &raw, 2);
-      const uint32_t o = (u & 0x8000u) ? (~(uint32_t)u & 0xffffu) : (u | 0x8000u);
-      lo[j] = c > -INFINITY ? (o << 16 | low) : 0u;
+      uint32_t u;                      // the 16 bits of the logit, on top
+      if constexpr (Elem<T>::dtype == D2DMOE_F16) u = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)c) << 16;
+      else u = __float_as_uint(c);
+      const uint32_t o = (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) & 0xffff0000u;
+      lo[j] = c > -INFINITY ? (o | low) : 0u;
     }
   }
   __device__ __forceinline__ void order(int i, int k) {   // larger key to place i
@@ -250,7 +252,7 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
 }
 
 // The choice on float64 scores, with the waves' slow way of finding a maximum: returns place tl's expert (or -1).
-template <int V, int L>
+template <int V, int L, bool GROUPS>
 __device__ __forceinline__ int choose_exactly(const float (&z)[V], const RouteArgs& A, bool row_bad, double* lds) {
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), e0 = tl * V;
   const double low = -(double)INFINITY;
@@ -273,7 +275,7 @@ __device__ __forceinline__ int choose_exactly(const float (&z)[V], const RouteAr
     if (A.bias != nullptr && e0 + j < A.E) by[j] += (double)A.bias[e0 + j];
     by[j] = (z[j] == -INFINITY || row_bad) ? low : by[j] + 0.0;
   }
-  if (A.G > 1) keep_groups<double, V, L>(by, A, 0.0, 0.0, lds, lds + 64 / L * A.E);
+  if constexpr (GROUPS) keep_groups<double, V, L>(by, A, 0.0, 0.0, lds, lds + 64 / L * A.E);
   int place = -1;
   for (int i = 0; i < A.K; ++i) {
     double v = low;
@@ -295,37 +297,42 @@ __device__ __forceinline__ int choose_exactly(const float (&z)[V], const RouteAr
   return place;
 }
 
-// DIRECT: the choice goes by the logits themselves (an instance of its own: without the float64 choice it needs 60 registers
-// less, and the order of the scores is that of the logits, so nothing is in doubt).
-template <typename T, int V, int L, bool DIRECT>
+// What the choice goes by, each an instance of its own: the logits (no score, no doubt, 32-bit keys for 16-bit types), scores
+// with a bias, or either of them within groups.
+enum { BY_LOGIT, BY_SCORE, IN_GROUPS };
+
+template <typename T, int V, int L, int MODE>
 __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restrict__ logits, T* __restrict__ routing, const RouteArgs A,
                                                                 int wave_lds) {
   extern __shared__ __align__(16) char lds_raw[];
   constexpr int TOK = 64 / L;
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
-  char* lds = lds_raw + (threadIdx.x >> 6) * wave_lds;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);    // uniform: rows and addresses are scalars
+  char* lds = lds_raw + wave * wave_lds;
   int* hist = (int*)(lds_raw + WAVES * wave_lds);
   if (A.counts != nullptr) {
     for (int e = threadIdx.x; e < A.E; e += WAVES * 64) hist[e] = 0;
     __syncthreads();
   }
-  constexpr bool direct = DIRECT;
-  const int have = A.E - e0;                             // experts from e0 on (<= 0: an idle lane)
+  const bool direct = MODE == BY_LOGIT || (MODE == IN_GROUPS && A.bias == nullptr && !A.top2);
+  const int have = A.E - e0;                                  // experts from e0 on (<= 0: an idle lane)
   const int64_t tiles = (A.N + TOK - 1) / TOK;
-  for (int64_t tile = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6); tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
-    const int64_t row = tile * TOK + team;
-    const bool live = row < A.N;
-    const T* zr = logits + row * A.E;
+  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
+    const int rows = (int)((A.N - tile * TOK < TOK) ? A.N - tile * TOK : TOK);
+    const bool live = team < rows;
+    const T* zt = logits + tile * TOK * A.E;                  // the wave's rows
+    const int row_at = team * A.E;
     float z[V];
-    load_run<V>(zr + e0, live ? have : 0, -INFINITY, z);
+    load_run<V>(zt + row_at + e0, live ? have : 0, -INFINITY, z);
     bool bad = false;
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      bad = bad || z[j] != z[j] || (A.softmax && z[j] == INFINITY);
+      bad = bad || z[j] != z[j];
       top = fmaxf(top, z[j]);
     }
-    const bool whole = A.softmax && !(A.renorm && direct);      // the row's softmax is needed, not only its order
+    if (A.softmax) bad = bad || top == INFINITY;
+    const bool whole = A.softmax && !(A.renorm && direct);    // the row's softmax is needed, not only its order
     float sum = 1.f;
     float p[V];
     if (whole) {
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       sum = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        p[j] = expf(z[j] - top);
+        p[j] = quick_exp(z[j] - top);
         sum += p[j];
       }
       sum = team_sum<L>(sum);
@@ -342,75 +349,80 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     float by[V];
     if (direct) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) by[j] = z[j] + 0.f;           // + 0: the two zeros are one value
+      for (int j = 0; j < V; ++j) by[j] = z[j] + 0.f;         // + 0: the two zeros are one value
     } else {
+      const float inv = __builtin_amdgcn_rcpf(sum);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float c = A.softmax ? p[j] / sum : 1.f / (1.f + expf(-z[j]));
+        float c = A.softmax ? p[j] * inv : __builtin_amdgcn_rcpf(1.f + quick_exp(-z[j]));
         if (A.bias != nullptr && j < have) c += A.bias[e0 + j];
         by[j] = z[j] == -INFINITY ? -INFINITY : c + 0.f;
         bad = bad || by[j] != by[j];
       }
     }
     bad = team_any<L>(bad);
-    if (bad) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) by[j] = -INFINITY;
-    }
+    for (int j = 0; j < V; ++j) by[j] = bad ? -INFINITY : by[j];
     bool doubt = false;
-    if (A.G > 1)
+    if constexpr (MODE == IN_GROUPS)
       doubt = keep_groups<float, V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
-    using K = Keys<T, V, !DIRECT || sizeof(T) == 4>;
+    using K = Keys<T, V, MODE != BY_LOGIT || sizeof(T) == 4>;
     K keys;
 #pragma unroll
     for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
     keys.sort();
-    uint32_t mine_hi = 0, mine_lo = 0;                          // place tl's key
+    uint32_t mine_hi = 0, mine_lo = 0;                        // place tl's key
     float last = 0.f;
-    const int turns = direct ? A.K : A.K + 1;                   // one more where the runner-up may be too close
+    const int turns = direct ? A.K : A.K + 1;                 // one more where the runner-up may be too close
     for (int i = 0; i < turns; ++i) {
       uint32_t hi, lo;
       keys.template take<L>(hi, lo);
       if (tl == i) { mine_hi = hi; mine_lo = lo; }
-      if (!direct) {
+      if (MODE != BY_LOGIT && !direct) {
         const float c = hi != 0 ? K::choice(hi) : -INFINITY;
         if (i > 0 && hi != 0 && last - c <= 0x1p-19f + 0x1p-22f * fabsf(last)) doubt = true;
         last = c;
       }
     }
     int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
-    if constexpr (!direct) {
-      if (__ballot(doubt) != 0ull) at = choose_exactly<V, L>(z, A, bad, (double*)lds);
+    if constexpr (MODE != BY_LOGIT) {
+      if (!direct && __ballot(doubt) != 0ull) at = choose_exactly<V, L, MODE == IN_GROUPS>(z, A, bad, (double*)lds);
     }
     // place tl's weight
     float zi = -INFINITY;
-    if (at >= 0) zi = direct ? K::choice(mine_hi) : Elem<T>::load(zr + at);
+    if (MODE == BY_LOGIT) {
+      if (at >= 0) zi = K::choice(mine_hi);
+    } else {
+      if (at >= 0) zi = Elem<T>::load(zt + row_at + at);
+    }
     float ref = A.softmax ? top : 0.f;
     if (A.renorm) {
       ref = team_max<L>(A.softmax ? zi : fminf(zi, 0.f));
       if (!finite(ref)) ref = 0.f;
     }
-    float w = 0.f;
-    if (at >= 0) w = A.softmax ? expf(zi - ref) : expf(fminf(zi, 0.f) - ref) / (1.f + expf(-fabsf(zi)));
+    float w = expf((A.softmax ? zi : fminf(zi, 0.f)) - ref);
+    if (!A.softmax) w = w / (1.f + expf(-fabsf(zi)));
+    if (at < 0) w = 0.f;
     float total = A.softmax ? sum : 1.f;
     if (A.renorm) total = team_sum<L>(w);
     w = at >= 0 ? A.scale * (w / total) : 0.f;
     if (tl < A.K && live) {
-      if (A.indices) A.indices[row * A.K + tl] = at;
-      if (A.weights) A.weights[row * A.K + tl] = w;
+      const int64_t first = tile * TOK * A.K;
+      const int o = team * A.K + tl;
+      if (A.indices) (A.indices + first)[o] = at;
+      if (A.weights) (A.weights + first)[o] = w;
       if (A.counts != nullptr && at >= 0) atomicAdd(hist + at, 1);
     }
     if (routing) {
-      T* dense = (T*)lds;                                       // [TOK][E], as the rows lie in memory
-      const int rows = (int)((A.N - tile * TOK < TOK) ? A.N - tile * TOK : TOK);
+      T* dense = (T*)lds;                                     // [TOK][E], as the rows lie in memory
+      constexpr int C = 16 / (int)sizeof(T);
       const int n = rows * A.E;
       wave_sync();
-      for (int i = lane * (16 / (int)sizeof(T)); i < TOK * A.E; i += 64 * (16 / (int)sizeof(T))) *(uint4*)(dense + i) = make_uint4(0, 0, 0, 0);
+      for (int i = lane * C; i < n; i += 64 * C) *(uint4*)(dense + i) = make_uint4(0, 0, 0, 0);
       wave_sync();
-      if (at >= 0) Elem<T>::store(dense + team * A.E + at, w);
+      if (at >= 0) Elem<T>::store(dense + row_at + at, w);
       wave_sync();
       T* out = routing + tile * TOK * A.E;
-      constexpr int C = 16 / (int)sizeof(T);
       for (int i = lane * C; i < n; i += 64 * C) {
         if (i + C <= n) {
           const uint4 v = *(const uint4*)(dense + i);
@@ -440,23 +452,25 @@ __global__ __launch_bounds__(WAVES * 64) void route_grad_team_kernel(const T* __
   constexpr int TOK = 64 / L;
   __shared__ __align__(16) float tiles_raw[WAVES][64 * V];
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
-  float* own = tiles_raw[threadIdx.x >> 6] + team * L * V;      // this token's row (L V >= E)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float* own = tiles_raw[wave] + team * L * V;                  // this token's row (L V >= E)
   const bool whole = softmax && !renorm;
   const int64_t tiles = (N + TOK - 1) / TOK;
-  for (int64_t tile = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6); tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
-    const int64_t row = tile * TOK + team;
-    const bool live = row < N;
-    int at = (live && tl < K) ? indices[row * K + tl] : -1;
+  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
+    const bool live = team < N - tile * TOK;
+    const int64_t row_first = tile * TOK * E, place_first = tile * TOK * K;
+    const int row_at = team * E, place = team * K + tl;
+    int at = (live && tl < K) ? (indices + place_first)[place] : -1;
     if (at >= E) at = -1;
     float zi = -INFINITY, q = 0.f;
     if (at >= 0) {
-      zi = Elem<T>::load(logits + row * E + at);
-      if (g_routing) q = Elem<T>::load(g_routing + row * E + at);
-      if (g_weights) q += g_weights[row * K + tl];
+      zi = Elem<T>::load(logits + row_first + row_at + at);
+      if (g_routing) q = Elem<T>::load(g_routing + row_first + row_at + at);
+      if (g_weights) q += (g_weights + place_first)[place];
     }
     float z[V], top = 0.f, sum = 1.f;
     if (whole) {
-      load_run<V>(logits + row * E + e0, live ? E - e0 : 0, -INFINITY, z);
+      load_run<V>(logits + row_first + row_at + e0, live ? E - e0 : 0, -INFINITY, z);
       top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < V; ++j) top = fmaxf(top, z[j]);
@@ -465,7 +479,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_grad_team_kernel(const T* __
       sum = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        z[j] = expf(z[j] - top);
+        z[j] = quick_exp(z[j] - top);
         sum += z[j];
       }
       sum = team_sum<L>(sum);
@@ -475,8 +489,9 @@ __global__ __launch_bounds__(WAVES * 64) void route_grad_team_kernel(const T* __
       ref = team_max<L>(softmax ? zi : fminf(zi, 0.f));
       if (!finite(ref)) ref = 0.f;
     }
-    float s = 0.f;
-    if (at >= 0) s = softmax ? expf(zi - ref) : expf(fminf(zi, 0.f) - ref) / (1.f + expf(-fabsf(zi)));
+    float s = expf((softmax ? zi : fminf(zi, 0.f)) - ref);
+    if (!softmax) s = s / (1.f + expf(-fabsf(zi)));
+    if (at < 0) s = 0.f;
     if (renorm) {
       sum = team_sum<L>(s);
       q -= __shfl(at >= 0 ? q : 0.f, lane & ~(L - 1), kWave);   // less the first place's: no effect but on the rounding
@@ -499,10 +514,11 @@ __global__ __launch_bounds__(WAVES * 64) void route_grad_team_kernel(const T* __
       v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
     }
     if (whole && some) {
+      const float common = scale * dot / sum;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] -= scale * (z[j] / sum) * dot;
+      for (int j = 0; j < V; ++j) v[j] -= z[j] * common;
     }
-    if (live && e0 < E) store_run<V>(grad + row * E + e0, E - e0, v);
+    if (live && e0 < E) store_run<V>(grad + row_first + row_at + e0, E - e0, v);
   }
 }
 
@@ -755,8 +771,8 @@ hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, 
   if (A.G > 1) wave = (size_t)(64 / L) * (A.E + A.G) * sizeof(double);
   wave = (wave + 15) / 16 * 16;
   const size_t lds = WAVES * wave + (A.counts ? (size_t)A.E * 4 : 0);
-  const bool direct = A.bias == nullptr && !(A.G > 1 && A.top2);
-  const auto kern = direct ? route_team_kernel<T, V, L, true> : route_team_kernel<T, V, L, false>;
+  const auto kern = A.G > 1 ? route_team_kernel<T, V, L, IN_GROUPS>
+                            : (A.bias ? route_team_kernel<T, V, L, BY_SCORE> : route_team_kernel<T, V, L, BY_LOGIT>);
   if (lds > (64u << 10)) {   // (E > 512 with hundreds of groups)
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
