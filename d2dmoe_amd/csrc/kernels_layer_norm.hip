@@ -193,11 +193,15 @@ struct NormBackward {
   int D;
 };
 
+// The column sums of grad_weight and grad_bias ride along: every thread owns its columns for all the rows it sees, so they
+// cost two accumulators per element and no traffic until the end.  Rows are requested one ahead (the workgroups are as many
+// as two per CU hold, so registers are plenty).
 template <typename T, typename P, int TPR, int CH>
-__global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_grad_kernel(const NormBackward A) {
-  constexpr int V = kVec<T>, ROWS = TPR < NT ? NT / TPR : 1;
+__global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void layer_norm_grad_kernel(const NormBackward A) {
+  constexpr int V = kVec<T>, ROWS = TPR < NT ? NT / TPR : 1, Q = 2 * CH * V / 4;
+  constexpr bool AHEAD = TPR < 1024;      // (1024 threads leave 128 registers each: the row is requested when it is due)
   __shared__ float buf[2][2][TPR / 64];
-  __shared__ float columns[ROWS > 1 ? 2 * TPR * CH * V : 1];
+  __shared__ float4 sums[ROWS > 1 ? ROWS / 2 : 1][ROWS > 1 ? Q : 1][64];
   int turn = 0;
   const int t = threadIdx.x % TPR;
   const int D = A.D;
@@ -208,25 +212,36 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_grad_kernel(co
   const int skip = over <= 0 ? 0 : (over >= V ? V : over);
   if (skip == V) at[CH - 1] = 0;
   else if (skip > 0) at[CH - 1] = D - V;
-  float w[CH][V], sw[CH][V], sb[CH][V];
+  float w[CH][V], cs[2][CH][V];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) { w[c][j] = 1.f; sw[c][j] = 0.f; sb[c][j] = 0.f; }
+    for (int j = 0; j < V; ++j) { w[c][j] = 1.f; cs[0][c][j] = 0.f; cs[1][c][j] = 0.f; }
     if (A.weight) load_params<P, V>((const P*)A.weight + at[c], w[c]);
   }
   const float inv_d = 1.f / (float)D;
   const int64_t step = (int64_t)gridDim.x * ROWS;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row < A.N; row += step) {
-    uint4 gr[CH], hr[CH], sr[CH];
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  uint4 gr[CH], hr[CH], sr[CH];
+  float m, r;
+  auto request = [&](int64_t k) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      gr[c] = load16((const T*)A.g + row * D + at[c]);
-      hr[c] = load16((const T*)A.h + row * D + at[c]);
-      if (A.gs) sr[c] = load16((const T*)A.gs + row * D + at[c]);
+      gr[c] = load16((const T*)A.g + k * D + at[c]);
+      hr[c] = load16((const T*)A.h + k * D + at[c]);
     }
-    const float m = A.mean[row], r = A.rstd[row];
+    m = A.mean[k];
+    r = A.rstd[k];
+  };
+  if (AHEAD && row < A.N) request(row);
+  for (; row < A.N; row += step) {
+    if (!AHEAD) request(row);
+    if (A.gs) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) sr[c] = load16((const T*)A.gs + row * D + at[c]);
+    }
     float g[CH][V], n[CH][V];
+    const float rs = r;
     float a = 0.f, b = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -234,15 +249,16 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_grad_kernel(co
       decode<T>(hr[c], n[c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        n[c][j] = (n[c][j] - m) * r;
-        sw[c][j] = fmaf(g[c][j], n[c][j], sw[c][j]);
-        sb[c][j] += g[c][j];
+        n[c][j] = (n[c][j] - m) * rs;
+        cs[0][c][j] = fmaf(g[c][j], n[c][j], cs[0][c][j]);
+        cs[1][c][j] += g[c][j];
         g[c][j] *= w[c][j];
         const float u = (c < CH - 1 || j >= skip) ? g[c][j] : 0.f;
         a += u;
         b = (c < CH - 1 || j >= skip) ? fmaf(u, n[c][j], b) : b;
       }
     }
+    if (AHEAD && row + step < A.N) request(row + step);
     row_sum<TPR>(a, b, buf, turn);
     a *= inv_d;
     b *= inv_d;
@@ -251,9 +267,21 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_grad_kernel(co
       for (int c = 0; c < CH; ++c) {
         float s[V];
         if (A.gs) decode<T>(sr[c], s);
+        if (!AHEAD) {                           // from the row's own registers once more, rather than held across the barrier
+          // (the empty asm makes them new values to the compiler, which would otherwise keep the decoded ones)
+          asm volatile("" : "+v"(gr[c].x), "+v"(gr[c].y), "+v"(gr[c].z), "+v"(gr[c].w));
+          asm volatile("" : "+v"(hr[c].x), "+v"(hr[c].y), "+v"(hr[c].z), "+v"(hr[c].w));
+          decode<T>(gr[c], g[c]);
+          decode<T>(hr[c], n[c]);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            n[c][j] = (n[c][j] - m) * rs;
+            g[c][j] *= w[c][j];
+          }
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float v = r * (g[c][j] - a - n[c][j] * b);
+          const float v = rs * (g[c][j] - a - n[c][j] * b);
           g[c][j] = A.gs ? v + s[j] : v;
         }
         if (c < CH - 1 || skip < V) store16((T*)A.grad + row * D + at[c], encode<T>(g[c]));
@@ -261,34 +289,45 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_grad_kernel(co
     }
   }
   if (A.partial == nullptr) return;
-  float* out = A.partial + (int64_t)blockIdx.x * 2 * D;
-  if constexpr (ROWS == 1) {
+  float* flat = &cs[0][0][0];
+  if constexpr (ROWS > 1) {
+    // the waves' sums: (0 + 2) + (1 + 3), through LDS in the lanes' own order
+    const int wave = threadIdx.x >> 6;
+    static_assert(ROWS == 4, "");
+    auto leave = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int q = 0; q < Q; ++q) sums[to][q][t] = make_float4(flat[4 * q], flat[4 * q + 1], flat[4 * q + 2], flat[4 * q + 3]);
+    };
+    auto add = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (c < CH - 1 || j >= skip) {
-          out[at[c] + j] = sw[c][j];
-          out[D + at[c] + j] = sb[c][j];
-        }
-  } else {
-    // the waves' sums one after the other, in wave order
-    for (int i = 0; i < ROWS; ++i) {
-      if ((int)threadIdx.x / TPR == i) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (c < CH - 1 || j >= skip) {
-              float* p = columns + at[c] + j;
-              p[0] = i == 0 ? sw[c][j] : p[0] + sw[c][j];
-              p[D] = i == 0 ? sb[c][j] : p[D] + sb[c][j];
-            }
+      for (int q = 0; q < Q; ++q) {
+        const float4 v = sums[from][q][t];
+        flat[4 * q] += v.x; flat[4 * q + 1] += v.y; flat[4 * q + 2] += v.z; flat[4 * q + 3] += v.w;
       }
-      __syncthreads();
-    }
-    for (int d = threadIdx.x; d < 2 * D; d += NT) out[d] = columns[d];
+    };
+    if (wave >= 2) leave(wave - 2);
+    __syncthreads();
+    if (wave < 2) add(wave);
+    __syncthreads();
+    if (wave == 1) leave(0);
+    __syncthreads();
+    if (wave != 0) return;
+    add(0);
   }
+  float* out = A.partial + (int64_t)blockIdx.x * 2 * D;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float* p = out + k * D + at[c];
+      if (c < CH - 1 || skip == 0) {
+        __builtin_memcpy(p, cs[k][c], sizeof(cs[k][c]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j >= skip) p[j] = cs[k][c][j];
+      }
+    }
 }
 
 // The workgroups' column sums added in a fixed order.  Workgroup = 32 of the 2 D columns, 32 threads per column: thread q adds
@@ -430,18 +469,20 @@ __global__ __launch_bounds__(NT) void layer_norm_grad_columns_kernel(const T* __
 
 inline int slab_count(int64_t N) { return (int)(N < 64 ? 1 : (cdiv64(N, 64) < 256 ? cdiv64(N, 64) : 256)); }
 
-// Threads per row and vectors per thread for a width, or TPR = 0 where the row does not fit.  Up to four vectors per thread
-// (32 16-bit values, with the column sums 160 registers); a wave per row as long as that is enough, then a workgroup.
+// Threads per row and vectors per thread for a width, or TPR = 0 where the row does not fit: a wave per row as long as `most`
+// vectors per thread are enough, then a workgroup.  Forward four; backward three, whose sums and the row ahead
+// make 228 of the 256 registers that two workgroups per CU leave each thread.
 struct RowPlan { int tpr, ch; };
-template <typename T> RowPlan row_plan(int D) {
+template <typename T> RowPlan row_plan(int D, int most) {
   constexpr int V = kVec<T>;
   if (D < V) return {0, 0};
   const int vectors = (D + V - 1) / V;
-  if (vectors <= 64 * 4) return {64, (vectors + 63) / 64};
-  if (vectors <= 256 * 4) return {256, (vectors + 255) / 256};
-  if (vectors <= 1024 * 2) return {1024, 2};
+  if (vectors <= 64 * most) return {64, (vectors + 63) / 64};
+  if (vectors <= 256 * most) return {256, (vectors + 255) / 256};
+  if (vectors <= 1024 * 2) return {1024, (vectors + 1023) / 1024};
   return {0, 0};
 }
+constexpr int kForwardVectors = 4, kBackwardVectors = 3;
 
 // Workgroups of the row kernels: enough to fill the machine's 256 CUs, each with as many rows as that leaves it.  (A constant:
 // the workspace and the order of the column sums depend on it.)
@@ -449,7 +490,8 @@ inline unsigned row_grid(int64_t N, int rows, int per_cu) {
   const int64_t need = cdiv64(N, rows), most = (int64_t)256 * per_cu;
   return (unsigned)(need < most ? need : most);
 }
-inline int grad_parts(const d2dmoe_norm_shape& sh, int tpr) { return (int)row_grid(sh.n_rows, tpr < NT ? NT / tpr : 1, tpr == 1024 ? 1 : 2); }
+// The gradient's: every workgroup leaves 2 D sums behind, so each takes four rows per wave or row team at least.
+inline int grad_parts(const d2dmoe_norm_shape& sh, int tpr) { return (int)row_grid(sh.n_rows, 4 * (tpr < NT ? NT / tpr : 1), tpr == 1024 ? 1 : 2); }
 
 template <typename T, typename P, int TPR, int CH>
 hipError_t forward_rows(const NormForward& A, hipStream_t s) {
@@ -466,27 +508,28 @@ hipError_t backward_rows(const NormBackward& A, unsigned grid, hipStream_t s) {
   return hipGetLastError();
 }
 
-#define D2DMOE_ROW_DISPATCH(PLAN, CALL)             \
+#define D2DMOE_ROW_DISPATCH(PLAN, CALL, EXTRA)      \
   switch (PLAN.tpr * 8 + PLAN.ch) {                 \
     case 64 * 8 + 1: e = CALL(64, 1); break;        \
     case 64 * 8 + 2: e = CALL(64, 2); break;        \
     case 64 * 8 + 3: e = CALL(64, 3); break;        \
-    case 64 * 8 + 4: e = CALL(64, 4); break;        \
+    case 256 * 8 + 1: e = CALL(256, 1); break;      \
     case 256 * 8 + 2: e = CALL(256, 2); break;      \
     case 256 * 8 + 3: e = CALL(256, 3); break;      \
-    case 256 * 8 + 4: e = CALL(256, 4); break;      \
+    case 1024 * 8 + 1: e = CALL(1024, 1); break;    \
+    EXTRA                                           \
     default: e = CALL(1024, 2); break;              \
   }
 
 template <typename T, typename P>
 hipError_t forward_t(const d2dmoe_norm_shape& sh, const void* x, const void* residual, const void* weight, const void* bias, void* sum,
                      void* out, float* mean, float* rstd, hipStream_t s) {
-  const RowPlan plan = row_plan<T>(sh.width);
+  const RowPlan plan = row_plan<T>(sh.width, kForwardVectors);
   hipError_t e;
   if (plan.tpr != 0) {
     const NormForward A{x, residual, weight, bias, sum, out, mean, rstd, sh.n_rows, sh.width, sh.eps};
 #define D2DMOE_ROWS(TPR, CH) forward_rows<T, P, TPR, CH>(A, s)
-    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS)
+    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, case 64 * 8 + 4: e = D2DMOE_ROWS(64, 4); break; case 256 * 8 + 4: e = D2DMOE_ROWS(256, 4); break;)
 #undef D2DMOE_ROWS
     return e;
   }
@@ -504,12 +547,12 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
   const bool columns = gw != nullptr || gb != nullptr;
   int parts = 0;                       // partial column sums in the workspace
   hipError_t e = hipSuccess;
-  const RowPlan plan = row_plan<T>(D);
+  const RowPlan plan = row_plan<T>(D, kBackwardVectors);
   if (N > 0 && plan.tpr != 0) {
     parts = grad_parts(sh, plan.tpr);
     const NormBackward A{g, gs, h, weight, mean, rstd, grad, columns ? (float*)workspace : nullptr, N, D};
 #define D2DMOE_ROWS(TPR, CH) backward_rows<T, P, TPR, CH>(A, (unsigned)parts, s)
-    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS)
+    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, )
 #undef D2DMOE_ROWS
   } else if (N > 0) {
     if (grad != nullptr) {
@@ -535,7 +578,7 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
 
 size_t layer_norm_workspace_bytes(const d2dmoe_norm_shape& sh) {
   if (sh.n_rows <= 0) return 0;
-  const RowPlan plan = sh.dtype == D2DMOE_F32 ? row_plan<float>(sh.width) : row_plan<bf16_t>(sh.width);
+  const RowPlan plan = sh.dtype == D2DMOE_F32 ? row_plan<float>(sh.width, kBackwardVectors) : row_plan<bf16_t>(sh.width, kBackwardVectors);
   const int parts = plan.tpr != 0 ? grad_parts(sh, plan.tpr) : slab_count(sh.n_rows);
   return (size_t)parts * 2 * sh.width * sizeof(float);
 }

@@ -177,7 +177,13 @@ __device__ inline void store_run(T* p, int count, const float (&v)[V]) {
 struct RouteArgs {
   const float* bias; int32_t* indices; float* weights; int32_t* counts;
   int64_t N; int E, K, softmax, G, kept, top2, renorm; float scale;
+  int size;                             // experts per group
+  float inv_size, inv_G, inv_lanes;     // 1 / size, 1 / G, 1 / (lanes per group) where groups are whole lanes
 };
+
+// a / b for 0 <= a < 4096 and b <= 1024 from a float32 1 / b: (a + 1/2) / b is at least 1 / (2 b) away from a whole number, the
+// product's error below 4096 * 2^-22
+__device__ inline int small_div(int a, float inv_b) { return (int)(((float)a + 0.5f) * inv_b); }
 
 // Drops the groups that do not stay from by[] (-inf).  `near`: how close two scores may lie for their order to be in doubt
 // (0: exact); returns whether one was.  tile: T E values, score: T G values of the wave's own LDS (C units).
@@ -185,7 +191,7 @@ template <typename C, int V, int L>
 __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_rel, C* tile, C* score) {
   constexpr int T = 64 / L;
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L;
-  const int size = A.E / A.G, G = A.G, e0 = tl * V;
+  const int size = A.size, G = A.G, e0 = tl * V;
   const C low = -(C)INFINITY;
   wave_sync();
   if (size % V == 0) {
@@ -196,7 +202,7 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
       b = larger(b, smaller(a, by[j]));
       a = larger(a, by[j]);
     }
-    const int lanes = size / V, pos = tl % lanes;
+    const int lanes = size / V, of = small_div(tl, A.inv_lanes), pos = tl - of * lanes;
     for (int off = 1; off < lanes; off <<= 1) {
       const C oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
       if (pos + off < lanes) {
@@ -204,7 +210,7 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
         a = larger(a, oa);
       }
     }
-    if (pos == 0 && e0 < A.E) score[team * G + tl / lanes] = (A.top2 && b > low) ? a + b : a;
+    if (pos == 0 && e0 < A.E) score[team * G + of] = (A.top2 && b > low) ? a + b : a;
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -225,8 +231,8 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
   bool doubt = false;
   uint8_t* stays = (uint8_t*)tile;
   for (int p = lane; p < T * G; p += 64) {
-    const C* all = score + p / G * G;
-    const int g = p % G;
+    const int first = small_div(p, A.inv_G) * G, g = p - first;
+    const C* all = score + first;
     const C mine = all[g];
     const C size_of = mine < 0 ? -mine : mine;
     const C near_by = (near_abs > 0 && size_of < (C)INFINITY) ? near_abs + near_rel * size_of : (C)0;
@@ -241,7 +247,7 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
     stays[p] = ahead < A.kept ? 1 : 0;
   }
   wave_sync();
-  int g = e0 / size, r = e0 - g * size;
+  int g = small_div(e0, A.inv_size), r = e0 - g * size;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     if (e0 + j < A.E && !stays[team * G + g]) by[j] = low;
@@ -352,10 +358,12 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       for (int j = 0; j < V; ++j) by[j] = z[j] + 0.f;         // + 0: the two zeros are one value
     } else {
       const float inv = __builtin_amdgcn_rcpf(sum);
+      float b[V];
+      if (A.bias != nullptr) load_run<V>(A.bias + e0, have, 0.f, b);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float c = A.softmax ? p[j] * inv : __builtin_amdgcn_rcpf(1.f + quick_exp(-z[j]));
-        if (A.bias != nullptr && j < have) c += A.bias[e0 + j];
+        if (A.bias != nullptr) c += b[j];
         by[j] = z[j] == -INFINITY ? -INFINITY : c + 0.f;
         bad = bad || by[j] != by[j];
       }
@@ -393,7 +401,13 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     if (MODE == BY_LOGIT) {
       if (at >= 0) zi = K::choice(mine_hi);
     } else {
-      if (at >= 0) zi = Elem<T>::load(zt + row_at + at);
+      // the chosen logits come out of the lanes that hold them through LDS
+      float* zs = (float*)lds + team * (L * V);
+      wave_sync();
+#pragma unroll
+      for (int j = 0; j < V; j += 4) *(float4*)(zs + e0 + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+      wave_sync();
+      if (at >= 0) zi = zs[at];
     }
     float ref = A.softmax ? top : 0.f;
     if (A.renorm) {
@@ -768,7 +782,8 @@ template <typename T, int V, int L>
 hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, const RouteArgs& A, hipStream_t s) {
   // per wave: the dense tile, and with groups the choices and the groups' scores in float64 (the exact choice's)
   size_t wave = (size_t)(64 / L) * A.E * sizeof(T);
-  if (A.G > 1) wave = (size_t)(64 / L) * (A.E + A.G) * sizeof(double);
+  if (A.G > 1 || A.bias) wave = (size_t)64 * V * sizeof(float);      // (the chosen logits)
+  if (A.G > 1 && wave < (size_t)(64 / L) * (A.E + A.G) * sizeof(double)) wave = (size_t)(64 / L) * (A.E + A.G) * sizeof(double);
   wave = (wave + 15) / 16 * 16;
   const size_t lds = WAVES * wave + (A.counts ? (size_t)A.E * 4 : 0);
   const auto kern = A.G > 1 ? route_team_kernel<T, V, L, IN_GROUPS>
@@ -787,7 +802,8 @@ hipError_t forward_t(const d2dmoe_route_shape& sh, const void* logits, const flo
   const int softmax = sh.scoring == D2DMOE_SCORE_SOFTMAX, top2 = sh.group_score == D2DMOE_GROUP_TOP2;
   if (sh.k <= 64) {
     const RouteArgs A{bias, indices, weights, counts, sh.n_tokens, sh.n_experts, sh.k, softmax, sh.n_groups, sh.kept_groups, top2,
-                      sh.renormalise, sh.scale};
+                      sh.renormalise, sh.scale, sh.n_experts / sh.n_groups, (float)sh.n_groups / (float)sh.n_experts,
+                      1.f / (float)sh.n_groups, (sh.n_experts > 512 ? 16.f : 8.f) * (float)sh.n_groups / (float)sh.n_experts};
     const T* z = (const T*)logits;
     T* r = (T*)routing;
     if (sh.n_experts > 512) return forward_l<T, 16, 64>(sh, z, r, A, s);
