@@ -185,51 +185,12 @@ struct RouteArgs {
 // product's error below 4096 * 2^-22
 __device__ inline int small_div(int a, float inv_b) { return (int)(((float)a + 0.5f) * inv_b); }
 
-// Drops the groups that do not stay from by[] (-inf).  `near`: how close two scores may lie for their order to be in doubt
-// (0: exact); returns whether one was.  tile: T E values, score: T G values of the wave's own LDS (C units).
-template <typename C, int V, int L>
-__device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_rel, C* tile, C* score) {
-  constexpr int T = 64 / L;
-  const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L;
-  const int size = A.size, G = A.G, e0 = tl * V;
-  const C low = -(C)INFINITY;
-  wave_sync();
-  if (size % V == 0) {
-    // whole lanes per group: the two largest of ever longer runs of lanes, up to the group's end, in its first lane
-    C a = low, b = low;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      b = larger(b, smaller(a, by[j]));
-      a = larger(a, by[j]);
-    }
-    const int lanes = size / V, of = small_div(tl, A.inv_lanes), pos = tl - of * lanes;
-    for (int off = 1; off < lanes; off <<= 1) {
-      const C oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
-      if (pos + off < lanes) {
-        b = larger(larger(b, ob), smaller(a, oa));
-        a = larger(a, oa);
-      }
-    }
-    if (pos == 0 && e0 < A.E) score[team * G + of] = (A.top2 && b > low) ? a + b : a;
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j < A.E) tile[team * A.E + e0 + j] = by[j];
-    wave_sync();
-    for (int p = lane; p < T * G; p += 64) {
-      const C* q = tile + p * size;       // team-major, groups in order: p counts both
-      C a = low, b = low;
-      for (int i = 0; i < size; ++i) {
-        const C v = q[i];
-        b = larger(b, smaller(a, v));
-        a = larger(a, v);
-      }
-      score[p] = (A.top2 && b > low) ? a + b : a;
-    }
-  }
-  wave_sync();
+// Which of the T G groups of a wave's tokens stay, from their scores: flags in stays[].  `near`: how close two scores may lie
+// for their order to be in doubt (0: exact); returns whether one was.
+template <typename C, int T>
+__device__ __forceinline__ bool rank_groups(const C* score, uint8_t* stays, const RouteArgs& A, C near_abs, C near_rel) {
+  const int lane = threadIdx.x & 63, G = A.G;
   bool doubt = false;
-  uint8_t* stays = (uint8_t*)tile;
   for (int p = lane; p < T * G; p += 64) {
     const int first = small_div(p, A.inv_G) * G, g = p - first;
     const C* all = score + first;
@@ -243,9 +204,64 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
       surely += (v > mine + near_by) ? 1 : 0;
       maybe += (o != g && v >= mine - near_by) ? 1 : 0;
     }
-    if (near_abs > 0 && mine > low && surely < A.kept && maybe >= A.kept) doubt = true;
+    if (near_abs > 0 && mine > -(C)INFINITY && surely < A.kept && maybe >= A.kept) doubt = true;
     stays[p] = ahead < A.kept ? 1 : 0;
   }
+  return __ballot(doubt) != 0ull;
+}
+
+// The scores of the T G groups from the choices in tile[] (T rows of E).
+template <typename C, int T>
+__device__ __forceinline__ void score_groups(const C* tile, C* score, const RouteArgs& A) {
+  const C low = -(C)INFINITY;
+  for (int p = threadIdx.x & 63; p < T * A.G; p += 64) {
+    const C* q = tile + p * A.size;       // token-major, groups in order: p counts both
+    C a = low, b = low;
+    for (int i = 0; i < A.size; ++i) {
+      const C v = q[i];
+      b = larger(b, smaller(a, v));
+      a = larger(a, v);
+    }
+    score[p] = (A.top2 && b > low) ? a + b : a;
+  }
+}
+
+// Drops the groups that do not stay from by[] (-inf); returns whether a group's place was in doubt.  tile: T E values, score:
+// T G values of the wave's own LDS.
+template <int V, int L>
+__device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, float near_abs, float near_rel, float* tile, float* score) {
+  constexpr int T = 64 / L;
+  const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L;
+  const int size = A.size, G = A.G, e0 = tl * V;
+  const float low = -INFINITY;
+  wave_sync();
+  if (size % V == 0) {
+    // whole lanes per group: the two largest of ever longer runs of lanes, up to the group's end, in its first lane
+    float a = low, b = low;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      b = larger(b, smaller(a, by[j]));
+      a = larger(a, by[j]);
+    }
+    const int lanes = size / V, of = small_div(tl, A.inv_lanes), pos = tl - of * lanes;
+    for (int off = 1; off < lanes; off <<= 1) {
+      const float oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
+      if (pos + off < lanes) {
+        b = larger(larger(b, ob), smaller(a, oa));
+        a = larger(a, oa);
+      }
+    }
+    if (pos == 0 && e0 < A.E) score[team * G + of] = (A.top2 && b > low) ? a + b : a;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < A.E) tile[team * A.E + e0 + j] = by[j];
+    wave_sync();
+    score_groups<float, T>(tile, score, A);
+  }
+  wave_sync();
+  uint8_t* stays = (uint8_t*)tile;
+  const bool doubt = rank_groups<float, T>(score, stays, A, near_abs, near_rel);
   wave_sync();
   int g = small_div(e0, A.inv_size), r = e0 - g * size;
 #pragma unroll
@@ -254,51 +270,70 @@ __device__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_r
     if (++r == size) { r = 0; ++g; }
   }
   wave_sync();
-  return __ballot(doubt) != 0ull;
+  return doubt;
 }
 
-// The choice on float64 scores, with the waves' slow way of finding a maximum: returns place tl's expert (or -1).
-template <int V, int L, bool GROUPS>
-__device__ __forceinline__ int choose_exactly(const float (&z)[V], const RouteArgs& A, bool row_bad, double* lds) {
-  const int lane = threadIdx.x & 63, tl = lane & (L - 1), e0 = tl * V;
+// The choice on float64 scores: returns place tl's expert (or -1).  Rare, so written for few registers rather than speed (the
+// kernel's occupancy is set by its widest part): the choices live in LDS -- tile[] of T rows of E, score[] of T rows of G and
+// T G flags behind it -- and no loop is unrolled.
+template <typename T, int V, int L, bool GROUPS>
+__device__ __forceinline__ int choose_exactly(const T* zr, bool live, bool row_bad, const RouteArgs& A, double* tiles) {
+  constexpr int TOK = 64 / L;
+  const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
+  const int end = e0 + V < A.E ? e0 + V : A.E;
   const double low = -(double)INFINITY;
-  double by[V];
+  double* tile = tiles + team * A.E;
+  double* score = tiles + TOK * A.E;
+  wave_sync();
   float top = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < V; ++j) top = fmaxf(top, z[j]);
-  top = team_max<L>(top);
-  if (!finite(top)) top = 0.f;
-  double total = 0.0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    by[j] = A.softmax ? exp((double)z[j] - (double)top) : 1.0 / (1.0 + exp(-(double)z[j]));
-    total += by[j];
+  double total = 1.0;
+  if (A.softmax) {
+#pragma unroll 1
+    for (int e = e0; e < end; ++e) top = fmaxf(top, live ? Elem<T>::load(zr + e) : -INFINITY);
+    top = team_max<L>(top);
+    if (!finite(top)) top = 0.f;
+    total = 0.0;
+#pragma unroll 1
+    for (int e = e0; e < end; ++e) total += live ? exp((double)Elem<T>::load(zr + e) - (double)top) : 0.0;
+    total = team_sum<L>(total);
   }
-  if (A.softmax) total = team_sum<L>(total);
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (A.softmax) by[j] /= total;
-    if (A.bias != nullptr && e0 + j < A.E) by[j] += (double)A.bias[e0 + j];
-    by[j] = (z[j] == -INFINITY || row_bad) ? low : by[j] + 0.0;
+#pragma unroll 1
+  for (int e = e0; e < end; ++e) {
+    const float z = live ? Elem<T>::load(zr + e) : -INFINITY;
+    const double x = exp(A.softmax ? (double)z - (double)top : -(double)z);
+    double c = A.softmax ? x / total : 1.0 / (1.0 + x);
+    if (A.bias != nullptr) c += (double)A.bias[e];
+    tile[e] = (z == -INFINITY || row_bad) ? low : c + 0.0;
   }
-  if constexpr (GROUPS) keep_groups<double, V, L>(by, A, 0.0, 0.0, lds, lds + 64 / L * A.E);
+  wave_sync();
+  if constexpr (GROUPS) {
+    uint8_t* stays = (uint8_t*)(score + TOK * A.G);
+    score_groups<double, TOK>(tiles, score, A);
+    wave_sync();
+    rank_groups<double, TOK>(score, stays, A, 0.0, 0.0);
+    wave_sync();
+#pragma unroll 1
+    for (int e = e0; e < end; ++e)
+      if (!stays[team * A.G + small_div(e, A.inv_size)]) tile[e] = low;
+    wave_sync();
+  }
   int place = -1;
+#pragma unroll 1
   for (int i = 0; i < A.K; ++i) {
     double v = low;
     int at = MAX_E;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (by[j] > v) { v = by[j]; at = e0 + j; }
-#pragma unroll
+#pragma unroll 1
+    for (int e = e0; e < end; ++e)
+      if (tile[e] > v) { v = tile[e]; at = e; }
+#pragma unroll 1
     for (int off = 1; off < L; off <<= 1) {
       const double ov = __shfl_xor(v, off, kWave);
       const int oa = __shfl_xor(at, off, kWave);
       if (ov > v || (ov == v && oa < at)) { v = ov; at = oa; }
     }
     if (tl == i) place = v > low ? at : -1;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j == at) by[j] = low;
+    if (at >= e0 && at < end) tile[at] = low;
+    wave_sync();
   }
   return place;
 }
@@ -322,8 +357,8 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
   }
   const bool direct = MODE == BY_LOGIT || (MODE == IN_GROUPS && A.bias == nullptr && !A.top2);
   const int have = A.E - e0;                                  // experts from e0 on (<= 0: an idle lane)
-  const int64_t tiles = (A.N + TOK - 1) / TOK;
-  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
+  const int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
+  if (tile * TOK < A.N) {
     const int rows = (int)((A.N - tile * TOK < TOK) ? A.N - tile * TOK : TOK);
     const bool live = team < rows;
     const T* zt = logits + tile * TOK * A.E;                  // the wave's rows
@@ -373,7 +408,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     for (int j = 0; j < V; ++j) by[j] = bad ? -INFINITY : by[j];
     bool doubt = false;
     if constexpr (MODE == IN_GROUPS)
-      doubt = keep_groups<float, V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
+      doubt = keep_groups<V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
     using K = Keys<T, V, MODE != BY_LOGIT || sizeof(T) == 4>;
     K keys;
 #pragma unroll
@@ -394,7 +429,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     }
     int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
     if constexpr (MODE != BY_LOGIT) {
-      if (!direct && __ballot(doubt) != 0ull) at = choose_exactly<V, L, MODE == IN_GROUPS>(z, A, bad, (double*)lds);
+      if (!direct && __ballot(doubt) != 0ull) at = choose_exactly<T, V, L, MODE == IN_GROUPS>(zt + row_at, live, bad, A, (double*)lds);
     }
     // place tl's weight
     float zi = -INFINITY;
@@ -469,8 +504,8 @@ __global__ __launch_bounds__(WAVES * 64) void route_grad_team_kernel(const T* __
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float* own = tiles_raw[wave] + team * L * V;                  // this token's row (L V >= E)
   const bool whole = softmax && !renorm;
-  const int64_t tiles = (N + TOK - 1) / TOK;
-  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * WAVES) {
+  const int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
+  if (tile * TOK < N) {
     const bool live = team < N - tile * TOK;
     const int64_t row_first = tile * TOK * E, place_first = tile * TOK * K;
     const int row_at = team * E, place = team * K + tl;
@@ -773,27 +808,39 @@ inline int team_lanes(int E, int V, int K) {
   return lanes;
 }
 
-inline unsigned team_grid(int64_t N, int L) {
-  const int64_t blocks = cdiv64(cdiv64(N, 64 / L), WAVES);
-  return (unsigned)(blocks < 4096 ? blocks : 4096);
-}
+// One tile per wave, no loop over tiles: the compiler would move what a tile computes from E and the lane out of it and hold
+// it in registers (130 to 160 of them, three waves per SIMD instead of five).  More workgroups than one launch takes (2^32
+// work-items) go in slices of 2^22.
+constexpr int64_t SLICE = (int64_t)1 << 22;
+inline int64_t team_blocks(int64_t N, int L) { return cdiv64(cdiv64(N, 64 / L), WAVES); }
 
 template <typename T, int V, int L>
 hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, const RouteArgs& A, hipStream_t s) {
-  // per wave: the dense tile, and with groups the choices and the groups' scores in float64 (the exact choice's)
-  size_t wave = (size_t)(64 / L) * A.E * sizeof(T);
-  if (A.G > 1 || A.bias) wave = (size_t)64 * V * sizeof(float);      // (the chosen logits)
-  if (A.G > 1 && wave < (size_t)(64 / L) * (A.E + A.G) * sizeof(double)) wave = (size_t)(64 / L) * (A.E + A.G) * sizeof(double);
+  // per wave: the dense tile; with scores the exact choice's T E values, and the chosen logits; with groups also T G scores and flags
+  const size_t tok = 64 / L;
+  size_t wave = tok * A.E * sizeof(T);
+  if (A.G > 1 || A.bias) wave = tok * A.E * sizeof(double) > 64 * V * sizeof(float) ? tok * A.E * sizeof(double) : 64 * V * sizeof(float);
+  if (A.G > 1) wave += tok * A.G * (sizeof(double) + 1);
   wave = (wave + 15) / 16 * 16;
   const size_t lds = WAVES * wave + (A.counts ? (size_t)A.E * 4 : 0);
   const auto kern = A.G > 1 ? route_team_kernel<T, V, L, IN_GROUPS>
                             : (A.bias ? route_team_kernel<T, V, L, BY_SCORE> : route_team_kernel<T, V, L, BY_LOGIT>);
-  if (lds > (64u << 10)) {   // (E > 512 with hundreds of groups)
+  if (lds > (64u << 10)) {   // (E near 1024 with hundreds of groups)
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(kern, dim3(team_grid(sh.n_tokens, L)), dim3(WAVES * 64), lds, s, logits, routing, A, (int)wave);
-  return hipGetLastError();
+  constexpr int64_t tokens = SLICE * WAVES * (64 / L);
+  for (int64_t done = 0; done < A.N; done += tokens) {
+    RouteArgs part = A;
+    part.N = A.N - done < tokens ? A.N - done : tokens;
+    if (A.indices) part.indices += done * A.K;
+    if (A.weights) part.weights += done * A.K;
+    hipLaunchKernelGGL(kern, dim3((unsigned)team_blocks(part.N, L)), dim3(WAVES * 64), lds, s, logits + done * A.E,
+                       routing ? routing + done * A.E : routing, part, (int)wave);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T>
@@ -824,10 +871,18 @@ hipError_t forward_t(const d2dmoe_route_shape& sh, const void* logits, const flo
 template <typename T, int V, int L>
 hipError_t backward_l(const d2dmoe_route_shape& sh, const void* logits, const int32_t* indices, const void* g_routing,
                       const float* g_weights, void* grad, hipStream_t s) {
-  hipLaunchKernelGGL((route_grad_team_kernel<T, V, L>), dim3(team_grid(sh.n_tokens, L)), dim3(WAVES * 64), 0, s, (const T*)logits, indices,
-                     (const T*)g_routing, g_weights, (T*)grad, sh.n_tokens, sh.n_experts, sh.k, sh.scoring == D2DMOE_SCORE_SOFTMAX,
-                     sh.renormalise, sh.scale);
-  return hipGetLastError();
+  constexpr int64_t tokens = SLICE * WAVES * (64 / L);
+  const int E = sh.n_experts, K = sh.k;
+  for (int64_t done = 0; done < sh.n_tokens; done += tokens) {
+    const int64_t n = sh.n_tokens - done < tokens ? sh.n_tokens - done : tokens;
+    hipLaunchKernelGGL((route_grad_team_kernel<T, V, L>), dim3((unsigned)team_blocks(n, L)), dim3(WAVES * 64), 0, s,
+                       (const T*)logits + done * E, indices + done * K, g_routing ? (const T*)g_routing + done * E : nullptr,
+                       g_weights ? g_weights + done * K : nullptr, (T*)grad + done * E, n, E, K, sh.scoring == D2DMOE_SCORE_SOFTMAX,
+                       sh.renormalise, sh.scale);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T>

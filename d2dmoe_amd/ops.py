@@ -378,13 +378,17 @@ def forward(x: torch.Tensor, router_w1: Optional[torch.Tensor], router_w2: Optio
 
 
 # ---- layer norm and routing by scores --------------------------------------------------------------------------------
+# the handle of a device's current stream (torch.cuda.current_stream builds a Stream object around it: 2.7 us of a 12 us call)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _launch(dev: torch.device, fn, what: str, *args) -> None:
     """One library call on the tensors' device and that device's current stream."""
     if dev.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+        status = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+            status = fn(*args, _raw_stream(dev.index))
     if status != 0:
         abi.check(status, what)
 

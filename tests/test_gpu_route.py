@@ -179,6 +179,24 @@ def test_no_tokens_and_many():
     del z, routing, grad
 
 
+def test_more_tokens_than_one_launch_takes():
+    """Sixteen tokens per wave, four waves per workgroup: the launches are cut at 2^22 workgroups."""
+    ops = _ops()
+    n = (1 << 28) + 77
+    z = torch.zeros(n, 4, dtype=torch.bfloat16, device=DEV)
+    z[:, 2] = 1.0
+    tail = _logits(100, 4, torch.bfloat16, seed=8)
+    z[-100:] = tail.to(DEV)
+    routing, indices, weights, counts = ops.route_topk(z, 1, 'sigmoid', renormalise=False, want_counts=True)
+    _check(tail, 1, 'sigmoid', None, dict(renormalise=False), torch.bfloat16, (routing[-100:], indices[-100:], weights[-100:], None))
+    assert (indices[:-100] == 2).all() and int(counts.sum()) == n
+    grad = ops.route_topk_backward(z, indices, 'sigmoid', False, grad_weights=torch.ones_like(weights))
+    assert (grad[:-100, 2] == grad[0, 2]).all() and not grad[:-100, 3].any()
+    ref = R.route_grads(tail.double().numpy(), indices[-100:].cpu().numpy(), np.ones((100, 1)), 'sigmoid', False, 1.0)
+    assert np.abs(grad[-100:].double().cpu().numpy() - ref).max() <= _half(torch.bfloat16)
+    del z, routing, indices, weights, grad
+
+
 def test_places_that_are_no_experts_are_left_out():
     """Indices of the caller's own making: out of range counts as left over, the same expert twice adds up."""
     z = _logits(6, 40, torch.float32, seed=2)
