@@ -273,67 +273,86 @@ __device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, 
   return doubt;
 }
 
-// The choice on float64 scores: returns place tl's expert (or -1).  Rare, so written for few registers rather than speed (the
-// kernel's occupancy is set by its widest part): the choices live in LDS -- tile[] of T rows of E, score[] of T rows of G and
-// T G flags behind it -- and no loop is unrolled.
-template <typename T, int V, int L, bool GROUPS>
-__device__ __forceinline__ int choose_exactly(const T* zr, bool live, bool row_bad, const RouteArgs& A, double* tiles) {
+// The choice on float64 scores: returns place tl's expert (or -1).  Few waves come here, but a launch waits for its last one,
+// and the kernel's occupancy is set by its widest part.  So: one exponential at a time (eight interleaved take 100 registers),
+// from LDS to LDS, then the choices in registers and the maxima over the team by lane permutes, as in the float32 choice.
+// tiles[]: T rows of E, T rows of G scores, T G flags.
+template <int V, int L, bool GROUPS>
+__device__ __forceinline__ int choose_exactly(const float (&z)[V], bool row_bad, const RouteArgs& A, double* tiles) {
   constexpr int TOK = 64 / L;
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
   const int end = e0 + V < A.E ? e0 + V : A.E;
   const double low = -(double)INFINITY;
   double* tile = tiles + team * A.E;
-  double* score = tiles + TOK * A.E;
   wave_sync();
   float top = -INFINITY;
-  double total = 1.0;
-  if (A.softmax) {
-#pragma unroll 1
-    for (int e = e0; e < end; ++e) top = fmaxf(top, live ? Elem<T>::load(zr + e) : -INFINITY);
-    top = team_max<L>(top);
-    if (!finite(top)) top = 0.f;
-    total = 0.0;
-#pragma unroll 1
-    for (int e = e0; e < end; ++e) total += live ? exp((double)Elem<T>::load(zr + e) - (double)top) : 0.0;
-    total = team_sum<L>(total);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (e0 + j < A.E) tile[e0 + j] = (double)z[j];
+    top = fmaxf(top, z[j]);
   }
+  top = team_max<L>(top);
+  if (!finite(top)) top = 0.f;
+  double total = 0.0;
 #pragma unroll 1
   for (int e = e0; e < end; ++e) {
-    const float z = live ? Elem<T>::load(zr + e) : -INFINITY;
-    const double x = exp(A.softmax ? (double)z - (double)top : -(double)z);
-    double c = A.softmax ? x / total : 1.0 / (1.0 + x);
-    if (A.bias != nullptr) c += (double)A.bias[e];
-    tile[e] = (z == -INFINITY || row_bad) ? low : c + 0.0;
+    const double v = tile[e];
+    const double x = exp(A.softmax ? v - (double)top : -v);
+    tile[e] = A.softmax ? x : 1.0 / (1.0 + x);
+    total += x;
   }
-  wave_sync();
+  if (A.softmax) total = team_sum<L>(total);
+  double by[V];
+  float b[V];
+  if (A.bias != nullptr) load_run<V>(A.bias + e0, A.E - e0, 0.f, b);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    double c = e0 + j < A.E ? tile[e0 + j] : 0.0;
+    if (A.softmax) c /= total;
+    if (A.bias != nullptr) c += (double)b[j];
+    by[j] = (z[j] == -INFINITY || row_bad) ? low : c + 0.0;
+  }
   if constexpr (GROUPS) {
+    double* score = tiles + TOK * A.E;
     uint8_t* stays = (uint8_t*)(score + TOK * A.G);
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < A.E) tile[e0 + j] = by[j];
+    wave_sync();
     score_groups<double, TOK>(tiles, score, A);
     wave_sync();
     rank_groups<double, TOK>(score, stays, A, 0.0, 0.0);
     wave_sync();
-#pragma unroll 1
-    for (int e = e0; e < end; ++e)
-      if (!stays[team * A.G + small_div(e, A.inv_size)]) tile[e] = low;
-    wave_sync();
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < A.E && !stays[team * A.G + small_div(e0 + j, A.inv_size)]) by[j] = low;
   }
   int place = -1;
 #pragma unroll 1
   for (int i = 0; i < A.K; ++i) {
     double v = low;
     int at = MAX_E;
-#pragma unroll 1
-    for (int e = e0; e < end; ++e)
-      if (tile[e] > v) { v = tile[e]; at = e; }
-#pragma unroll 1
-    for (int off = 1; off < L; off <<= 1) {
-      const double ov = __shfl_xor(v, off, kWave);
-      const int oa = __shfl_xor(at, off, kWave);
-      if (ov > v || (ov == v && oa < at)) { v = ov; at = oa; }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double c = by[j];
+      at = c > v ? e0 + j : at;
+      v = larger(v, c);
     }
-    if (tl == i) place = v > low ? at : -1;
-    if (at >= e0 && at < end) tile[at] = low;
-    wave_sync();
+    // the team's largest: order-preserving halves, then the lowest index
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint64_t o = u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
+    const uint32_t h = team_max_u<L>((uint32_t)(o >> 32));
+    const bool first = (uint32_t)(o >> 32) == h;
+    const uint32_t m = team_max_u<L>(first ? (uint32_t)o : 0u);
+    const uint32_t l = team_max_u<L>((first && (uint32_t)o == m && v > low) ? (uint32_t)(2 * MAX_E - at) : 0u);
+    const int best = l != 0u ? 2 * MAX_E - (int)l : -1;
+    if (tl == i) place = best;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double c = by[j];
+      by[j] = e0 + j == best ? low : c;
+    }
   }
   return place;
 }
@@ -429,7 +448,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     }
     int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
     if constexpr (MODE != BY_LOGIT) {
-      if (!direct && __ballot(doubt) != 0ull) at = choose_exactly<T, V, L, MODE == IN_GROUPS>(zt + row_at, live, bad, A, (double*)lds);
+      if (!direct && __ballot(doubt) != 0ull) at = choose_exactly<V, L, MODE == IN_GROUPS>(z, bad, A, (double*)lds);
     }
     // place tl's weight
     float zi = -INFINITY;
