@@ -628,7 +628,7 @@ int d2dmoe_route_topk(const d2dmoe_route_shape* shape, const void* logits, const
   if (st != D2DMOE_OK) return st;
   if (shape->n_tokens == 0 && !counts) return D2DMOE_OK;
   if (!routing && !indices && !weights && !counts) return D2DMOE_E_NULL;
-  if (shape->n_tokens > 0 && !logits) return D2DMOE_E_NULL;
+  if (shape->n_tokens > 0 && (!logits || (counts && !indices))) return D2DMOE_E_NULL;
   if (!aligned_elem(logits, shape->dtype) || !aligned_elem(routing, shape->dtype) || !aligned_elem(choice_bias, D2DMOE_F32) ||
       !aligned_elem(indices, D2DMOE_F32) || !aligned_elem(weights, D2DMOE_F32) || !aligned_elem(counts, D2DMOE_F32))
     return D2DMOE_E_ALIGN;

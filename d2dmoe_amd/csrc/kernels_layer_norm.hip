@@ -340,7 +340,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_finish_kernel(const floa
   const int d = (int)blockIdx.x * 32 + c;
   float s = 0.f;
   if (d < 2 * D) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = q; i < parts; i += 32) s += partial[(int64_t)i * 2 * D + d];
   }
   part[q][c] = s;

@@ -369,11 +369,8 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L, e0 = tl * V;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);    // uniform: rows and addresses are scalars
   char* lds = lds_raw + wave * wave_lds;
-  int* hist = (int*)(lds_raw + WAVES * wave_lds);
-  if (A.counts != nullptr) {
-    for (int e = threadIdx.x; e < A.E; e += WAVES * 64) hist[e] = 0;
-    __syncthreads();
-  }
+  if (A.counts != nullptr && blockIdx.x == 0)                 // (filled by the pass over the indices behind this launch)
+    for (int e = threadIdx.x; e < A.E; e += WAVES * 64) A.counts[e] = 0;
   const bool direct = MODE == BY_LOGIT || (MODE == IN_GROUPS && A.bias == nullptr && !A.top2);
   const int have = A.E - e0;                                  // experts from e0 on (<= 0: an idle lane)
   const int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
@@ -434,17 +431,17 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
     keys.sort();
     uint32_t mine_hi = 0, mine_lo = 0;                        // place tl's key
-    float last = 0.f;
-    const int turns = direct ? A.K : A.K + 1;                 // one more where the runner-up may be too close
-    for (int i = 0; i < turns; ++i) {
-      uint32_t hi, lo;
+    uint32_t hi = 0, lo;
+    for (int i = 0; i < A.K; ++i) {
       keys.template take<L>(hi, lo);
       if (tl == i) { mine_hi = hi; mine_lo = lo; }
-      if (MODE != BY_LOGIT && !direct) {
-        const float c = hi != 0 ? K::choice(hi) : -INFINITY;
-        if (i > 0 && hi != 0 && last - c <= 0x1p-19f + 0x1p-22f * fabsf(last)) doubt = true;
-        last = c;
-      }
+    }
+    if (MODE != BY_LOGIT && !direct) {
+      // places next to each other, and the last one with the first that was left out
+      keys.template take<L>(hi, lo);
+      const uint32_t next = tl == A.K - 1 ? hi : (uint32_t)__shfl_down((int)mine_hi, 1, kWave);
+      const float c = K::choice(mine_hi), d = K::choice(next);
+      if (tl < A.K && next != 0 && c - d <= 0x1p-19f + 0x1p-22f * fabsf(c)) doubt = true;
     }
     int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
     if constexpr (MODE != BY_LOGIT) {
@@ -479,7 +476,6 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       const int o = team * A.K + tl;
       if (A.indices) (A.indices + first)[o] = at;
       if (A.weights) (A.weights + first)[o] = w;
-      if (A.counts != nullptr && at >= 0) atomicAdd(hist + at, 1);
     }
     if (routing) {
       T* dense = (T*)lds;                                     // [TOK][E], as the rows lie in memory
@@ -502,11 +498,20 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       wave_sync();
     }
   }
-  if (A.counts != nullptr) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < A.E; e += WAVES * 64)
-      if (hist[e] != 0) atomicAdd(A.counts + e, hist[e]);
+}
+
+// Tokens per expert from the indices.  Integers, so the order of the additions does not show.
+__global__ __launch_bounds__(256) void route_count_kernel(const int32_t* __restrict__ indices, int64_t n, int32_t* __restrict__ counts, int E) {
+  __shared__ int hist[MAX_E];
+  for (int e = threadIdx.x; e < E; e += 256) hist[e] = 0;
+  __syncthreads();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int at = indices[i];
+    if (at >= 0) atomicAdd(hist + at, 1);
   }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += 256)
+    if (hist[e] != 0) atomicAdd(counts + e, hist[e]);
 }
 
 // Gradient by the same teams: lane i has place i (expert, score, gradient), the places' gradients meet in an LDS tile of the
@@ -601,6 +606,8 @@ __global__ __launch_bounds__(64) void route_kernel(const T* __restrict__ logits,
   __shared__ int s_idx[MAX_E];
   const int lane = threadIdx.x;
   const bool direct = bias == nullptr && !(G > 1 && top2);
+  if (counts != nullptr && blockIdx.x == 0)
+    for (int e = lane; e < E; e += 64) counts[e] = 0;
   for (int64_t row = blockIdx.x; row < N; row += gridDim.x) {
     const T* zr = logits + row * E;
     float z[PER_LANE];
@@ -697,7 +704,6 @@ __global__ __launch_bounds__(64) void route_kernel(const T* __restrict__ logits,
       if (lane == 0) {
         s_idx[i] = there ? at : -1;
         s_z[i] = there ? Elem<T>::load(zr + at) : -INFINITY;
-        if (there && counts != nullptr) atomicAdd(counts + at, 1);
       }
 #pragma unroll
       for (int j = 0; j < PER_LANE; ++j)
@@ -841,7 +847,7 @@ hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, 
   if (A.G > 1 || A.bias) wave = tok * A.E * sizeof(double) > 64 * V * sizeof(float) ? tok * A.E * sizeof(double) : 64 * V * sizeof(float);
   if (A.G > 1) wave += tok * A.G * (sizeof(double) + 1);
   wave = (wave + 15) / 16 * 16;
-  const size_t lds = WAVES * wave + (A.counts ? (size_t)A.E * 4 : 0);
+  const size_t lds = WAVES * wave;
   const auto kern = A.G > 1 ? route_team_kernel<T, V, L, IN_GROUPS>
                             : (A.bias ? route_team_kernel<T, V, L, BY_SCORE> : route_team_kernel<T, V, L, BY_LOGIT>);
   if (lds > (64u << 10)) {   // (E near 1024 with hundreds of groups)
@@ -927,15 +933,17 @@ hipError_t backward_t(const d2dmoe_route_shape& sh, const void* logits, const in
 
 hipError_t launch_route_topk(const d2dmoe_route_shape& sh, const void* logits, const float* bias, void* routing, int32_t* indices,
                              float* weights, int32_t* counts, hipStream_t s) {
-  if (counts != nullptr) {
-    const hipError_t e = launch_fill_i32(counts, sh.n_experts, 0, s);
-    if (e != hipSuccess || sh.n_tokens == 0) return e;
-  }
+  if (sh.n_tokens == 0) return counts ? launch_fill_i32(counts, sh.n_experts, 0, s) : hipSuccess;
+  hipError_t e;
   switch (sh.dtype) {
-    case D2DMOE_F32: return forward_t<float>(sh, logits, bias, routing, indices, weights, counts, s);
-    case D2DMOE_BF16: return forward_t<bf16_t>(sh, logits, bias, routing, indices, weights, counts, s);
-    default: return forward_t<f16_t>(sh, logits, bias, routing, indices, weights, counts, s);
+    case D2DMOE_F32: e = forward_t<float>(sh, logits, bias, routing, indices, weights, counts, s); break;
+    case D2DMOE_BF16: e = forward_t<bf16_t>(sh, logits, bias, routing, indices, weights, counts, s); break;
+    default: e = forward_t<f16_t>(sh, logits, bias, routing, indices, weights, counts, s); break;
   }
+  if (e != hipSuccess || counts == nullptr) return e;
+  const int64_t n = sh.n_tokens * sh.k, blocks = cdiv64(n, 1024);
+  hipLaunchKernelGGL(route_count_kernel, dim3((unsigned)(blocks < 256 ? blocks : 256)), dim3(256), 0, s, indices, n, counts, sh.n_experts);
+  return hipGetLastError();
 }
 
 hipError_t launch_route_topk_backward(const d2dmoe_route_shape& sh, const void* logits, const int32_t* indices, const void* g_routing,

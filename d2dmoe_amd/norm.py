@@ -36,7 +36,7 @@ class NormModes:
         if self._hip(x):
             return functional.layer_norm(x, self.weight, self.bias, self.norm_eps(), residual)
         h = x if residual is None else x + residual
-        out = F.layer_norm(h, self.weight.shape, self.weight, self.bias, self.norm_eps())
+        out = F.layer_norm(h, (h.size(-1),), self.weight, self.bias, self.norm_eps())
         return out if residual is None else (out, h)
 
 

@@ -393,20 +393,20 @@ def _launch(dev: torch.device, fn, what: str, *args) -> None:
         abi.check(status, what)
 
 
-def _norm_params(what: str, d: int, dtype: torch.dtype, **params: Optional[torch.Tensor]) -> int:
-    """Element type code of weight and bias (the activations' type, or float32); both have to agree."""
-    kind = None
-    for name, p in params.items():
+def _norm_params(what: str, d: int, dtype: torch.dtype, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None) -> int:
+    """Element type code of weight and bias: the activations' type, or float32; both have to agree."""
+    kind = dtype
+    for p in (weight, bias):
         if p is None:
             continue
-        if p.shape != (d,):
-            raise abi.D2DMoEError(f'{what}: {name} has shape {tuple(p.shape)}, the rows are {d} wide')
-        if p.dtype != dtype and p.dtype != torch.float32:
-            raise abi.D2DMoEError(f'{what}: {name} is {p.dtype}; with {dtype} activations it is {dtype} or torch.float32')
-        if kind is not None and p.dtype != kind:
-            raise abi.D2DMoEError(f'{what}: weight and bias are of two element types')
+        if p.dim() != 1 or p.size(0) != d:
+            raise abi.D2DMoEError(f'{what}: a parameter has shape {tuple(p.shape)}, the rows are {d} wide')
         kind = p.dtype
-    return _DTYPES[dtype if kind is None else kind]
+        if kind != dtype and kind != torch.float32:
+            raise abi.D2DMoEError(f'{what}: a parameter is {kind}; with {dtype} activations it is {dtype} or torch.float32')
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise abi.D2DMoEError(f'{what}: weight is {weight.dtype}, bias {bias.dtype}; they have one element type')
+    return _DTYPES[kind]
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
@@ -421,7 +421,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     dev = _require_gpu(x, residual, weight, bias)
     lib = abi.load()
     n, d = x.shape
-    pcode = _norm_params('layer_norm', d, x.dtype, weight=weight, bias=bias)
+    pcode = _norm_params('layer_norm', d, x.dtype, weight, bias)
     out = torch.empty_like(x)
     total = None if residual is None else torch.empty_like(x)
     mean = rstd = None
@@ -452,7 +452,7 @@ def layer_norm_backward(grad_out: torch.Tensor, h: torch.Tensor, weight: Optiona
             raise abi.D2DMoEError(f'layer_norm_backward: {name} is {t.dtype} {tuple(t.shape)}, expected float32 ({n},)')
     dev = _require_gpu(h, grad_out, grad_sum, weight, mean, rstd)
     lib = abi.load()
-    pcode = _norm_params('layer_norm_backward', d, h.dtype, weight=weight)
+    pcode = _norm_params('layer_norm_backward', d, h.dtype, weight)
     ptype = weight.dtype if weight is not None else (param_dtype or h.dtype)
     if weight is None:
         if ptype != h.dtype and ptype != torch.float32:
@@ -494,13 +494,15 @@ def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bi
     float32 [N,k], counts int32 [E] or None); places left over hold index -1 and weight 0."""
     sh = _route_shape('route_topk', logits, k, scoring, renormalise, scale, n_groups, kept_groups, group_score)
     n, e = logits.shape
+    if not 1 <= k <= e:
+        raise abi.D2DMoEError(f'route_topk: k = {k} of {e} experts')
     if choice_bias is not None and (choice_bias.dtype != torch.float32 or choice_bias.shape != (e,)):
         raise abi.D2DMoEError(f'route_topk: choice_bias is {choice_bias.dtype} {tuple(choice_bias.shape)}, expected float32 ({e},)')
     dev = _require_gpu(logits, choice_bias)
     lib = abi.load()
     routing = torch.empty_like(logits)
-    indices = torch.empty(n, max(k, 0), dtype=torch.int32, device=dev)
-    weights = torch.empty(n, max(k, 0), dtype=torch.float32, device=dev)
+    indices = torch.empty(n, k, dtype=torch.int32, device=dev)
+    weights = torch.empty(n, k, dtype=torch.float32, device=dev)
     counts = torch.empty(e, dtype=torch.int32, device=dev) if want_counts else None
     _launch(dev, lib.d2dmoe_route_topk, 'd2dmoe_route_topk', ctypes.byref(sh), logits.data_ptr(), _ptr(choice_bias),
             routing.data_ptr(), indices.data_ptr(), weights.data_ptr(), _ptr(counts))

@@ -351,7 +351,7 @@ typedef struct d2dmoe_route_shape {
 /*   choice_bias optional float32 [n_experts]
  *   routing optional T [n_tokens,n_experts]: the weights as the dense routing tensor every experts entry point takes
  *   indices optional int32 [n_tokens,k], weights optional float32 [n_tokens,k]: the same by place (-1 and 0 where a place is
- *   left over)      counts optional int32 [n_experts]: tokens per expert (zeroed here) */
+ *   left over)      counts optional int32 [n_experts]: tokens per expert (zeroed here; comes from `indices`, which it needs) */
 int d2dmoe_route_topk(const d2dmoe_route_shape* shape, const void* logits, const float* choice_bias, void* routing,
                       int32_t* indices, float* weights, int32_t* counts, void* stream);
 

@@ -213,7 +213,7 @@ def test_c_entry_points_refuse_before_anything_is_launched():
         return lib.d2dmoe_route_topk(ctypes.byref(rs), logits, bias, routing, indices, weights, counts, None)
 
     assert lib.d2dmoe_route_topk(None, p, None, p, p, p, None, None) == -1
-    assert route(logits=None) == route(routing=None, indices=None, weights=None) == -1
+    assert route(logits=None) == route(routing=None, indices=None, weights=None) == route(indices=None, counts=p) == -1
     assert route(n=-1) == route(e=0) == route(e=1025) == route(k=0) == route(k=9) == -2
     assert route(groups=3, kept=1) == route(groups=0) == route(groups=4, kept=5) == route(groups=4, kept=0) == -2
     assert route(groups=4, kept=1, k=3) == -2
