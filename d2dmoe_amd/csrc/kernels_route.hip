@@ -72,6 +72,7 @@ __device__ inline float from_order_bits(uint32_t o) { return __uint_as_float((o 
 // A lane's V choices as keys that compare as unsigned numbers, the larger choice first and the lower index first among equal
 // ones: 64 bits (order of a float32, index), or 32 where the choice is a 16-bit logit.
 template <typename T, int V, bool WIDE> struct Keys {
+  static constexpr bool kWide = WIDE;
   uint32_t hi[V], lo[V];   // narrow: lo alone
   __device__ __forceinline__ void set(int j, float c, int e) {
     const uint32_t low = (uint32_t)(2 * MAX_E - e);
@@ -109,15 +110,21 @@ template <typename T, int V, bool WIDE> struct Keys {
           for (int i = 0; i < (b < V - j - b ? b : V - j - b); ++i)
             if ((i + j) / (2 * a) == (i + j + b) / (2 * a)) order(i + j, i + j + b);
   }
-  // the team's largest key, which leaves its lane's list
-  template <int L> __device__ __forceinline__ void take(uint32_t& h, uint32_t& l) {
+  // The team's largest key, which leaves its lane's list.  Wide: h is its choice, and `won` the lane it was in -- the lowest of
+  // those whose list starts with that choice, and so with the lowest index -- found in scalar instructions: the lowest bit
+  // of each L-bit field of the ballot (no field is empty, so the subtraction does not borrow from the next).
+  template <int L> __device__ __forceinline__ void take(uint32_t& h, uint32_t& l, bool& won) {
     if constexpr (WIDE) {
+      constexpr uint64_t ones = L == 4 ? 0x1111111111111111ull : L == 8 ? 0x0101010101010101ull : L == 16 ? 0x0001000100010001ull
+                                                                      : L == 32 ? 0x0000000100000001ull : 1ull;
       h = team_max_u<L>(hi[0]);
-      l = team_max_u<L>(hi[0] == h ? lo[0] : 0u);
+      const uint64_t m = __ballot(hi[0] == h);
+      won = __builtin_amdgcn_inverse_ballot_w64(m & ~(m - ones));
+      l = lo[0];
     } else {
       h = l = team_max_u<L>(lo[0]);
+      won = lo[0] == l;
     }
-    const bool won = lo[0] == l;
 #pragma unroll
     for (int j = 0; j < V; ++j) {      // (values, not places, to choose from: the lists stay in registers)
       const uint32_t lc = lo[j], ln = j + 1 < V ? lo[j + 1 < V ? j + 1 : j] : 0u;
@@ -185,9 +192,10 @@ struct RouteArgs {
 // product's error below 4096 * 2^-22
 __device__ inline int small_div(int a, float inv_b) { return (int)(((float)a + 0.5f) * inv_b); }
 
-// Which of the T G groups of a wave's tokens stay, from their scores: flags in stays[].  `near`: how close two scores may lie
-// for their order to be in doubt (0: exact); returns whether one was.
-template <typename C, int T>
+// Which of the T G groups of a wave's tokens stay, from their scores: flags in stays[].  NEAR: scores closer than near_abs +
+// near_rel |score| leave the order in doubt; returns whether it was (the flags do not matter then).  Otherwise exact, ties to
+// the lowest group.
+template <typename C, int T, bool NEAR>
 __device__ __forceinline__ bool rank_groups(const C* score, uint8_t* stays, const RouteArgs& A, C near_abs, C near_rel) {
   const int lane = threadIdx.x & 63, G = A.G;
   bool doubt = false;
@@ -195,17 +203,28 @@ __device__ __forceinline__ bool rank_groups(const C* score, uint8_t* stays, cons
     const int first = small_div(p, A.inv_G) * G, g = p - first;
     const C* all = score + first;
     const C mine = all[g];
-    const C size_of = mine < 0 ? -mine : mine;
-    const C near_by = (near_abs > 0 && size_of < (C)INFINITY) ? near_abs + near_rel * size_of : (C)0;
-    int ahead = 0, surely = 0, maybe = 0;
-    for (int o = 0; o < G; ++o) {
-      const C v = all[o];
-      ahead += (v > mine || (v == mine && o < g)) ? 1 : 0;
-      surely += (v > mine + near_by) ? 1 : 0;
-      maybe += (o != g && v >= mine - near_by) ? 1 : 0;
+    if constexpr (NEAR) {
+      const C size_of = mine < 0 ? -mine : mine;
+      const C by = size_of < (C)INFINITY ? near_abs + near_rel * size_of : (C)0;
+      const C above = mine + by, below = mine - by;
+      int surely = 0, maybe = -1;                       // ahead of this one (which is within its own reach)
+#pragma unroll 4
+      for (int o = 0; o < G; ++o) {
+        const C v = all[o];
+        surely += v > above ? 1 : 0;
+        maybe += v >= below ? 1 : 0;
+      }
+      if (mine > -(C)INFINITY && surely < A.kept && maybe >= A.kept) doubt = true;
+      stays[p] = surely < A.kept ? 1 : 0;
+    } else {
+      int ahead = 0;
+#pragma unroll 4
+      for (int o = 0; o < G; ++o) {
+        const C v = all[o];
+        ahead += (v > mine || (v == mine && o < g)) ? 1 : 0;
+      }
+      stays[p] = ahead < A.kept ? 1 : 0;
     }
-    if (near_abs > 0 && mine > -(C)INFINITY && surely < A.kept && maybe >= A.kept) doubt = true;
-    stays[p] = ahead < A.kept ? 1 : 0;
   }
   return __ballot(doubt) != 0ull;
 }
@@ -261,13 +280,21 @@ __device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, 
   }
   wave_sync();
   uint8_t* stays = (uint8_t*)tile;
-  const bool doubt = rank_groups<float, T>(score, stays, A, near_abs, near_rel);
+  const bool doubt = near_abs > 0.f ? rank_groups<float, T, true>(score, stays, A, near_abs, near_rel)
+                                    : rank_groups<float, T, false>(score, stays, A, 0.f, 0.f);
   wave_sync();
-  int g = small_div(e0, A.inv_size), r = e0 - g * size;
+  int g = small_div(e0, A.inv_size);
+  if (size % V == 0) {
+    const bool out = e0 >= A.E || !stays[team * G + g];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (e0 + j < A.E && !stays[team * G + g]) by[j] = low;
-    if (++r == size) { r = 0; ++g; }
+    for (int j = 0; j < V; ++j) by[j] = out ? low : by[j];
+  } else {
+    int r = e0 - g * size;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (e0 + j < A.E && !stays[team * G + g]) by[j] = low;
+      if (++r == size) { r = 0; ++g; }
+    }
   }
   wave_sync();
   return doubt;
@@ -322,7 +349,7 @@ __device__ __forceinline__ int choose_exactly(const float (&z)[V], bool row_bad,
     wave_sync();
     score_groups<double, TOK>(tiles, score, A);
     wave_sync();
-    rank_groups<double, TOK>(score, stays, A, 0.0, 0.0);
+    rank_groups<double, TOK, false>(score, stays, A, 0.0, 0.0);
     wave_sync();
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -431,14 +458,28 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
     keys.sort();
     uint32_t mine_hi = 0, mine_lo = 0;                        // place tl's key
-    uint32_t hi = 0, lo;
+    uint32_t hi, lo;
+    bool won;
+    uint32_t* places = (uint32_t*)lds + team * A.K;           // wide keys: the winner's lane leaves its index here
+    if constexpr (K::kWide) wave_sync();
     for (int i = 0; i < A.K; ++i) {
-      keys.template take<L>(hi, lo);
-      if (tl == i) { mine_hi = hi; mine_lo = lo; }
+      keys.template take<L>(hi, lo, won);
+      if constexpr (K::kWide) {
+        if (won) places[i] = lo;
+        mine_hi = tl == i ? hi : mine_hi;
+      } else {
+        mine_lo = tl == i ? lo : mine_lo;
+      }
+    }
+    if constexpr (K::kWide) {
+      wave_sync();
+      if (tl < A.K) mine_lo = places[tl];
+    } else {
+      mine_hi = mine_lo;
     }
     if (MODE != BY_LOGIT && !direct) {
       // places next to each other, and the last one with the first that was left out
-      keys.template take<L>(hi, lo);
+      keys.template take<L>(hi, lo, won);
       const uint32_t next = tl == A.K - 1 ? hi : (uint32_t)__shfl_down((int)mine_hi, 1, kWave);
       const float c = K::choice(mine_hi), d = K::choice(next);
       if (tl < A.K && next != 0 && c - d <= 0x1p-19f + 0x1p-22f * fabsf(c)) doubt = true;
