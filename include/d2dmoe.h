@@ -294,7 +294,7 @@ int d2dmoe_expert_output_norms(const d2dmoe_shape* shape, const void* x, const v
 /* ---- layer norm --------------------------------------------------------------------------------------------------
  * Rows of h = x, or of h = x + residual rounded to T (the residual stream between a block's two halves):
  *   m = mean(h)   v = mean((h - m)^2)   r = 1 / sqrt(v + eps)   out = (h - m) r * weight + bias
- * Replaces the LayerNorm modules in front of a block's attention and FFN (architectures/gpt.py:27-36, 117-128) together
+ * Replaces the LayerNorm modules in front of a block's attention and FFN (architectures/gpt.py:27-36) together
  * with the residual addition ahead of the second one.  Statistics, sums and intermediates are float32; every stored
  * value is rounded once.  Any width, any element-aligned pointer.  Nothing may overlap an output. */
 typedef struct d2dmoe_norm_shape {
@@ -324,7 +324,7 @@ int d2dmoe_layer_norm_backward(const d2dmoe_norm_shape* shape, const void* grad_
 
 /* ---- routing by scores -------------------------------------------------------------------------------------------
  * The k experts of a token from a learned router's logits z, with weights: next to d2dmoe_select's dynamic-k rule, the
- * fixed-k rule of trained mixtures (and the weighted form of the reference's 'topk' gate, moefication.py:63-69).
+ * fixed-k rule of trained mixtures (and the weighted form of the reference's 'topk' gate, moefication.py:56-79).
  *   scores  s = softmax(z) or 1 / (1 + exp(-z))
  *   choice  c = s + choice_bias[e]; c = z where there is no bias and no sum of scores is needed (same order)
  *   groups  n_groups runs of n_experts / n_groups consecutive experts, a run scored by its largest c or by the sum of its
