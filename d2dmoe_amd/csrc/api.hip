@@ -590,7 +590,7 @@ int d2dmoe_layer_norm(const d2dmoe_norm_shape* shape, const void* x, const void*
   const int st = check_norm_shape(shape);
   if (st != D2DMOE_OK) return st;
   if (shape->n_rows == 0) return D2DMOE_OK;
-  if (!x || !out) return D2DMOE_E_NULL;
+  if (!x || !out || (sum && !residual)) return D2DMOE_E_NULL;
   const int t = shape->dtype, p = shape->param_dtype;
   if (!aligned_elem(x, t) || !aligned_elem(residual, t) || !aligned_elem(sum, t) || !aligned_elem(out, t) || !aligned_elem(weight, p) ||
       !aligned_elem(bias, p) || !aligned_elem(mean, D2DMOE_F32) || !aligned_elem(rstd, D2DMOE_F32))

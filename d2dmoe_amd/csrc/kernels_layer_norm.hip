@@ -7,8 +7,8 @@
 // All sums, the statistics and every intermediate are float32; what is stored in 16 bits is rounded once (h = x + residual
 // is such a value: it is the residual stream, an output, and the norm is taken of what the stream holds).
 //
-// Two kernels per direction: one that keeps a row in registers (any width up to 16384), one that passes over it again for
-// every use (wider rows, and rows narrower than one vector).
+// Two kernels per direction: one that keeps a row in registers (from one 16-byte vector up to 32768 16-bit or 16384 float32
+// values forward, half of that backward), one that passes over it again for every use (other widths).
 #include "launch.hpp"
 #include "mfma_common.hpp"
 #include "team.hpp"
@@ -20,15 +20,15 @@ namespace {
 constexpr int NT = 256;   // threads per workgroup
 
 // ---------------------------------------------------------------------------------------------------------------------
-// A row in registers.  TPR threads per row: one wave (four rows per workgroup, no barrier) or a whole workgroup, CH vectors
-// of 16 bytes each.  All but the last of the CH are whole; in the last one a thread may lie behind the row's end (it reads
+// A row in registers.  TPR threads per row: a part of a wave (8, 16 or 32 lanes: narrow rows, several per wave), one wave, or a
+// whole workgroup of 256 or 1024 (the only ones with a barrier), CH vectors of 16 bytes each.  All but the last of the CH are whole; in the last one a thread may lie behind the row's end (it reads
 // the row's first vector and drops it) or across it (it reads the row's last whole vector, of which it counts the elements
 // nobody else has; the others are computed twice and stored twice, with the same bits).  Rows may begin at any element: the
 // loads and stores make no claim on alignment.
 //
 // Bound by HBM: a row is read once and written once.  bf16 with residual, 50432 x 768: 60 us, 5.1 TB/s (this card copies at
-// 4.9 to 5.5 TB/s); 32768 x 4096 with statistics: 195 us, 5.5 TB/s.  With a pass over the row for each use it was 259 us for
-// the former, and one row per workgroup in all.
+// 4.9 to 5.5 TB/s); 32768 x 4096 with statistics: 195 us, 5.5 TB/s; 65536 x 64: 6.7 us, 5.0 TB/s.  With one row per workgroup
+// and a pass over it for each use the first was 259 us.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 
@@ -74,12 +74,13 @@ template <typename P, int V> __device__ __forceinline__ void load_params(const P
 
 // Sums of two values over the TPR threads of a row.  `turn` alternates between calls: the next call writes the other half of
 // buf, and the one after comes behind a barrier that every reader of this half has passed, so one barrier each is enough.
+template <int TPR> constexpr int kWaves = TPR > 64 ? TPR / 64 : 1;   // per row
 template <int TPR>
-__device__ __forceinline__ void row_sum(float& a, float& b, float (*buf)[2][TPR / 64], int& turn) {
-  a = team_sum<64>(a);
-  b = team_sum<64>(b);
+__device__ __forceinline__ void row_sum(float& a, float& b, float (*buf)[2][kWaves<TPR>], int& turn) {
+  a = team_sum<(TPR < 64 ? TPR : 64)>(a);
+  b = team_sum<(TPR < 64 ? TPR : 64)>(b);
   if constexpr (TPR > 64) {
-    float (*half)[TPR / 64] = buf[turn];
+    float (*half)[kWaves<TPR>] = buf[turn];
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) {
       half[0][threadIdx.x >> 6] = a;
@@ -95,6 +96,14 @@ __device__ __forceinline__ void row_sum(float& a, float& b, float (*buf)[2][TPR 
   }
 }
 
+// The rows of a workgroup: ROWS at a time, RPW of them per wave.  The loop over them is uniform for a wave: `row` is its first
+// one, and a lane whose own row lies behind the end works on the last row and stores nothing.
+template <int TPR> constexpr int kRows = TPR < NT ? NT / TPR : 1;
+template <int TPR> constexpr int kRowsPerWave = TPR < 64 ? 64 / TPR : 1;
+template <int TPR> __device__ __forceinline__ int64_t first_row() {
+  return (int64_t)blockIdx.x * kRows<TPR> + (TPR < NT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kRowsPerWave<TPR> : 0);
+}
+
 struct NormForward {
   const void *x, *residual, *weight, *bias;
   void *sum, *out;
@@ -106,8 +115,8 @@ struct NormForward {
 
 template <typename T, typename P, int TPR, int CH, bool RES>
 __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_kernel(const NormForward A) {
-  constexpr int V = kVec<T>, ROWS = TPR < NT ? NT / TPR : 1;
-  __shared__ float buf[2][2][TPR / 64];
+  constexpr int V = kVec<T>, RPW = kRowsPerWave<TPR>;
+  __shared__ float buf[2][2][kWaves<TPR>];
   int turn = 0;
   const int t = threadIdx.x % TPR;
   const int D = A.D;
@@ -127,18 +136,22 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_kernel(const N
     if (A.bias) load_params<P, V>((const P*)A.bias + at[c], b[c]);
   }
   const float inv_d = 1.f / (float)D;
-  const int64_t step = (int64_t)gridDim.x * ROWS;
-  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows<TPR>;
+  const int sub = RPW > 1 ? (threadIdx.x & 63) / TPR : 0;
   uint4 xr[CH], rr[CH];
-  auto request = [&](int64_t r) __attribute__((always_inline)) {
+  auto request = [&](int64_t wave_row) __attribute__((always_inline)) {
+    const int64_t r = RPW > 1 && wave_row + sub >= A.N ? A.N - 1 : wave_row + sub;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       xr[c] = load16((const T*)A.x + r * D + at[c]);
       if (RES) rr[c] = load16((const T*)A.residual + r * D + at[c]);
     }
   };
-  if (row < A.N) request(row);
-  for (; row < A.N; row += step) {
+  int64_t wave_row = first_row<TPR>();
+  if (wave_row < A.N) request(wave_row);
+  for (; wave_row < A.N; wave_row += step) {
+    const int64_t row = wave_row + sub;
+    const bool live = RPW == 1 || row < A.N;
     float h[CH][V];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -150,10 +163,10 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_kernel(const N
         for (int j = 0; j < V; ++j) h[c][j] += r[j];
         const uint4 packed = encode<T>(h[c]);               // the stream as it is stored is what the norm sees
         decode<T>(packed, h[c]);
-        if (A.sum && (c < CH - 1 || skip < V)) store16((T*)A.sum + row * D + at[c], packed);
+        if (A.sum && live && (c < CH - 1 || skip < V)) store16((T*)A.sum + row * D + at[c], packed);
       }
     }
-    if (row + step < A.N) request(row + step);              // the next row travels while this one is worked on
+    if (wave_row + step < A.N) request(wave_row + step);    // the next row travels while this one is worked on
     float s = 0.f, none = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -179,9 +192,9 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR) void layer_norm_kernel(const N
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
       for (int j = 0; j < V; ++j) h[c][j] = fmaf((h[c][j] - dm) * r, w[c][j], b[c][j]);
-      if (c < CH - 1 || skip < V) store16((T*)A.out + row * D + at[c], encode<T>(h[c]));
+      if (live && (c < CH - 1 || skip < V)) store16((T*)A.out + row * D + at[c], encode<T>(h[c]));
     }
-    if (t == 0) {
+    if (t == 0 && live) {
       if (A.mean) A.mean[row] = m + dm;
       if (A.rstd) A.rstd[row] = r;
     }
@@ -204,10 +217,10 @@ struct NormBackward {
 // many sums to finish) took the same time at 768 and 2 us more at 4097 x 1280, where they are too few to fill the machine.
 template <typename T, typename P, int TPR, int CH>
 __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void layer_norm_grad_kernel(const NormBackward A) {
-  constexpr int V = kVec<T>, ROWS = TPR < NT ? NT / TPR : 1, Q = 2 * CH * V / 4;
+  constexpr int V = kVec<T>, RPW = kRowsPerWave<TPR>, Q = 2 * CH * V / 4;
   constexpr bool AHEAD = TPR < 1024;      // (1024 threads leave 128 registers each: the row is requested when it is due)
-  __shared__ float buf[2][2][TPR / 64];
-  __shared__ float4 sums[ROWS > 1 ? ROWS / 2 : 1][ROWS > 1 ? Q : 1][64];
+  __shared__ float buf[2][2][kWaves<TPR>];
+  __shared__ float4 sums[TPR <= 64 ? 2 : 1][TPR <= 64 ? Q : 1][64];
   int turn = 0;
   const int t = threadIdx.x % TPR;
   const int D = A.D;
@@ -226,11 +239,12 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
     if (A.weight) load_params<P, V>((const P*)A.weight + at[c], w[c]);
   }
   const float inv_d = 1.f / (float)D;
-  const int64_t step = (int64_t)gridDim.x * ROWS;
-  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows<TPR>;
+  const int sub = RPW > 1 ? (threadIdx.x & 63) / TPR : 0;
   uint4 gr[CH], hr[CH], sr[CH];
   float m, r;
-  auto request = [&](int64_t k) __attribute__((always_inline)) {
+  auto request = [&](int64_t wave_row) __attribute__((always_inline)) {
+    const int64_t k = RPW > 1 && wave_row + sub >= A.N ? A.N - 1 : wave_row + sub;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       gr[c] = load16((const T*)A.g + k * D + at[c]);
@@ -239,9 +253,12 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
     m = A.mean[k];
     r = A.rstd[k];
   };
-  if (AHEAD && row < A.N) request(row);
-  for (; row < A.N; row += step) {
-    if (!AHEAD) request(row);
+  int64_t wave_row = first_row<TPR>();
+  if (AHEAD && wave_row < A.N) request(wave_row);
+  for (; wave_row < A.N; wave_row += step) {
+    if (!AHEAD) request(wave_row);
+    const bool live = RPW == 1 || wave_row + sub < A.N;
+    const int64_t row = live ? wave_row + sub : A.N - 1;
     if (A.gs) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) sr[c] = load16((const T*)A.gs + row * D + at[c]);
@@ -256,15 +273,15 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         n[c][j] = (n[c][j] - m) * rs;
-        cs[0][c][j] = fmaf(g[c][j], n[c][j], cs[0][c][j]);
-        cs[1][c][j] += g[c][j];
+        cs[0][c][j] = live ? fmaf(g[c][j], n[c][j], cs[0][c][j]) : cs[0][c][j];
+        cs[1][c][j] = live ? cs[1][c][j] + g[c][j] : cs[1][c][j];
         g[c][j] *= w[c][j];
         const float u = (c < CH - 1 || j >= skip) ? g[c][j] : 0.f;
         a += u;
         b = (c < CH - 1 || j >= skip) ? fmaf(u, n[c][j], b) : b;
       }
     }
-    if (AHEAD && row + step < A.N) request(row + step);
+    if (AHEAD && wave_row + step < A.N) request(wave_row + step);
     row_sum<TPR>(a, b, buf, turn);
     a *= inv_d;
     b *= inv_d;
@@ -290,24 +307,28 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
           const float v = rs * (g[c][j] - a - n[c][j] * b);
           g[c][j] = A.gs ? v + s[j] : v;
         }
-        if (c < CH - 1 || skip < V) store16((T*)A.grad + row * D + at[c], encode<T>(g[c]));
+        if (live && (c < CH - 1 || skip < V)) store16((T*)A.grad + row * D + at[c], encode<T>(g[c]));
       }
     }
   }
   if (A.partial == nullptr) return;
   float* flat = &cs[0][0][0];
-  if constexpr (ROWS > 1) {
+  if constexpr (TPR <= 64) {
+    // the wave's rows first, where it has several
+#pragma unroll
+    for (int off = TPR; off < 64; off <<= 1)
+#pragma unroll
+      for (int q = 0; q < 4 * Q; ++q) flat[q] += __shfl_xor(flat[q], off, kWave);
     // the waves' sums: (0 + 2) + (1 + 3), through LDS in the lanes' own order
-    const int wave = threadIdx.x >> 6;
-    static_assert(ROWS == 4, "");
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     auto leave = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) sums[to][q][t] = make_float4(flat[4 * q], flat[4 * q + 1], flat[4 * q + 2], flat[4 * q + 3]);
+      for (int q = 0; q < Q; ++q) sums[to][q][lane] = make_float4(flat[4 * q], flat[4 * q + 1], flat[4 * q + 2], flat[4 * q + 3]);
     };
     auto add = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        const float4 v = sums[from][q][t];
+        const float4 v = sums[from][q][lane];
         flat[4 * q] += v.x; flat[4 * q + 1] += v.y; flat[4 * q + 2] += v.z; flat[4 * q + 3] += v.w;
       }
     };
@@ -317,7 +338,7 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
     __syncthreads();
     if (wave == 1) leave(0);
     __syncthreads();
-    if (wave != 0) return;
+    if (wave != 0 || lane >= TPR) return;
     add(0);
   }
   float* out = A.partial + (int64_t)blockIdx.x * 2 * D;
@@ -475,20 +496,21 @@ __global__ __launch_bounds__(NT) void layer_norm_grad_columns_kernel(const T* __
 
 inline int slab_count(int64_t N) { return (int)(N < 64 ? 1 : (cdiv64(N, 64) < 256 ? cdiv64(N, 64) : 256)); }
 
-// Threads per row and vectors per thread for a width, or TPR = 0 where the row does not fit: a wave per row as long as `most`
-// vectors per thread are enough, then a workgroup.  Forward four; backward three, whose sums and the row ahead
-// make 228 of the 256 registers that two workgroups per CU leave each thread.
+// Threads per row and vectors per thread for a width, or TPR = 0 where the row does not fit: as few lanes as one vector each is
+// enough for (65536 rows of 64 bf16: 23 us with a wave each), then a wave per row as long as `most` vectors per thread are
+// enough, then a workgroup of 256, of 1024.  Forward four; backward three, whose sums and the row ahead make 228 of the 256
+// registers that two workgroups per CU leave each thread (1024 threads have 128, room for one, two with spills).
 struct RowPlan { int tpr, ch; };
-template <typename T> RowPlan row_plan(int D, int most) {
+template <typename T> RowPlan row_plan(int D, bool forward) {
   constexpr int V = kVec<T>;
   if (D < V) return {0, 0};
-  const int vectors = (D + V - 1) / V;
+  const int vectors = (D + V - 1) / V, most = forward ? 4 : 3;
+  if (vectors <= 32) return {vectors <= 8 ? 8 : vectors <= 16 ? 16 : 32, 1};
   if (vectors <= 64 * most) return {64, (vectors + 63) / 64};
   if (vectors <= 256 * most) return {256, (vectors + 255) / 256};
-  if (vectors <= 1024 * 2) return {1024, (vectors + 1023) / 1024};
+  if (vectors <= 1024 * (forward ? 4 : 2)) return {1024, (vectors + 1023) / 1024};
   return {0, 0};
 }
-constexpr int kForwardVectors = 4, kBackwardVectors = 3;
 
 // Workgroups of the row kernels: enough to fill the machine's 256 CUs, each with as many rows as that leaves it.  (A constant:
 // the workspace and the order of the column sums depend on it.)
@@ -502,7 +524,7 @@ inline int grad_parts(const d2dmoe_norm_shape& sh, int tpr) { return (int)row_gr
 template <typename T, typename P, int TPR, int CH>
 hipError_t forward_rows(const NormForward& A, hipStream_t s) {
   constexpr int threads = TPR < NT ? NT : TPR;
-  const unsigned grid = row_grid(A.N, TPR < NT ? NT / TPR : 1, TPR == 1024 ? 2 : 5);
+  const unsigned grid = row_grid(A.N, kRows<TPR>, TPR == 1024 ? 2 : 5);
   if (A.residual) hipLaunchKernelGGL((layer_norm_kernel<T, P, TPR, CH, true>), dim3(grid), dim3(threads), 0, s, A);
   else hipLaunchKernelGGL((layer_norm_kernel<T, P, TPR, CH, false>), dim3(grid), dim3(threads), 0, s, A);
   return hipGetLastError();
@@ -516,6 +538,9 @@ hipError_t backward_rows(const NormBackward& A, unsigned grid, hipStream_t s) {
 
 #define D2DMOE_ROW_DISPATCH(PLAN, CALL, EXTRA)      \
   switch (PLAN.tpr * 8 + PLAN.ch) {                 \
+    case 8 * 8 + 1: e = CALL(8, 1); break;          \
+    case 16 * 8 + 1: e = CALL(16, 1); break;        \
+    case 32 * 8 + 1: e = CALL(32, 1); break;        \
     case 64 * 8 + 1: e = CALL(64, 1); break;        \
     case 64 * 8 + 2: e = CALL(64, 2); break;        \
     case 64 * 8 + 3: e = CALL(64, 3); break;        \
@@ -530,12 +555,14 @@ hipError_t backward_rows(const NormBackward& A, unsigned grid, hipStream_t s) {
 template <typename T, typename P>
 hipError_t forward_t(const d2dmoe_norm_shape& sh, const void* x, const void* residual, const void* weight, const void* bias, void* sum,
                      void* out, float* mean, float* rstd, hipStream_t s) {
-  const RowPlan plan = row_plan<T>(sh.width, kForwardVectors);
+  const RowPlan plan = row_plan<T>(sh.width, true);
   hipError_t e;
   if (plan.tpr != 0) {
     const NormForward A{x, residual, weight, bias, sum, out, mean, rstd, sh.n_rows, sh.width, sh.eps};
 #define D2DMOE_ROWS(TPR, CH) forward_rows<T, P, TPR, CH>(A, s)
-    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, case 64 * 8 + 4: e = D2DMOE_ROWS(64, 4); break; case 256 * 8 + 4: e = D2DMOE_ROWS(256, 4); break;)
+    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, case 64 * 8 + 4: e = D2DMOE_ROWS(64, 4); break;
+                        case 256 * 8 + 4: e = D2DMOE_ROWS(256, 4); break; case 1024 * 8 + 3: e = D2DMOE_ROWS(1024, 3); break;
+                        case 1024 * 8 + 4: e = D2DMOE_ROWS(1024, 4); break;)
 #undef D2DMOE_ROWS
     return e;
   }
@@ -553,7 +580,7 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
   const bool columns = gw != nullptr || gb != nullptr;
   int parts = 0;                       // partial column sums in the workspace
   hipError_t e = hipSuccess;
-  const RowPlan plan = row_plan<T>(D, kBackwardVectors);
+  const RowPlan plan = row_plan<T>(D, false);
   if (N > 0 && plan.tpr != 0) {
     parts = grad_parts(sh, plan.tpr);
     const NormBackward A{g, gs, h, weight, mean, rstd, grad, columns ? (float*)workspace : nullptr, N, D};
@@ -584,7 +611,7 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
 
 size_t layer_norm_workspace_bytes(const d2dmoe_norm_shape& sh) {
   if (sh.n_rows <= 0) return 0;
-  const RowPlan plan = sh.dtype == D2DMOE_F32 ? row_plan<float>(sh.width, kBackwardVectors) : row_plan<bf16_t>(sh.width, kBackwardVectors);
+  const RowPlan plan = sh.dtype == D2DMOE_F32 ? row_plan<float>(sh.width, false) : row_plan<bf16_t>(sh.width, false);
   const int parts = plan.tpr != 0 ? grad_parts(sh, plan.tpr) : slab_count(sh.n_rows);
   return (size_t)parts * 2 * sh.width * sizeof(float);
 }

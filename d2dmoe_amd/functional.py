@@ -1,7 +1,11 @@
 """The operators of this package that have a backward pass, as differentiable functions on ROCm tensors: layer norm (with
 the residual added ahead of it) and routing by scores.  Forward and backward are the HIP kernels behind ``ops``; what is
 saved for the backward pass is the normalised tensor with its row statistics, or the logits with the chosen indices.
-Where no gradient is asked for, nothing is saved.  Double backward is not supported."""
+Where no gradient is asked for, nothing is saved.  Double backward is not supported.
+
+Capturing a training step into a HIP graph: PyTorch ties a parameter's gradient accumulator to the stream on which the first
+graph that reaches it was built, so capture before an eager graph of the same parameters is alive (or after it has been
+dropped), or call ``ops.layer_norm_backward`` / ``ops.route_topk_backward``, which take no part in autograd."""
 from __future__ import annotations
 
 from typing import Optional
@@ -71,6 +75,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise ops.abi.D2DMoEError(f'layer_norm: residual has shape {tuple(residual.shape)}, x {tuple(shape)}')
     x2 = x.reshape(-1, shape[-1]).contiguous()
     r2 = None if residual is None else residual.reshape(-1, shape[-1]).contiguous()
+    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
     if _wanted(x, residual, weight, bias):
         out, total = _LayerNorm.apply(x2, r2, weight, bias, eps)
     else:

@@ -202,6 +202,12 @@ class MoeficationMoE(MoELayer):
 
     SCORE_GATES = {'softmax_topk': 'softmax', 'sigmoid_topk': 'sigmoid'}
 
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        saved = state_dict.get(prefix + 'balance_bias')
+        if saved is not None and self.balance_bias is None:      # saved with one: the layer gets one
+            self.balance_bias = torch.empty_like(saved, device=next(self.parameters()).device)
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+
     # ------------------------------------------------------------------------------ gating
     def gate(self, x):
         mode = self.forward_mode
@@ -230,6 +236,8 @@ class MoeficationMoE(MoELayer):
             routing[norms >= thresholds] = 1.0
             return routing
         if mode in self.SCORE_GATES:
+            if self.k is None:
+                raise ValueError(f"forward_mode {mode!r} needs k, the number of experts per token")
             logits = self.router(x)
             bias = None if self.balance_bias is None else self.balance_bias.float()
             args = (self.k, self.SCORE_GATES[mode], bias, self.n_groups, self.kept_groups, self.group_score, self.renormalise,

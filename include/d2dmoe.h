@@ -305,7 +305,7 @@ typedef struct d2dmoe_norm_shape {
   float eps;            /* finite, >= 0 */
 } d2dmoe_norm_shape;
 
-/*   residual optional [n_rows,width]; sum optional: receives h (with a residual); weight, bias optional [width]
+/*   residual optional [n_rows,width]; sum optional, with a residual only: receives h; weight, bias optional [width]
  *   mean, rstd optional float32 [n_rows]: the row statistics, what the backward pass needs next to h */
 int d2dmoe_layer_norm(const d2dmoe_norm_shape* shape, const void* x, const void* residual, const void* weight, const void* bias,
                       void* sum, void* out, float* mean, float* rstd, void* stream);

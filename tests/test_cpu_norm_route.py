@@ -139,6 +139,13 @@ def test_layer_gates_by_scores_on_the_cpu():
     moe.balance_bias[6] = 10.0
     assert 'balance_bias' in moe.state_dict()
     assert (moe.gate(x)[..., 6] > 0).all()
+    fresh = MoeficationMoE('m', 16, 8, True, 4, torch.nn.ReLU)
+    fresh.router = MoeficationRouter(16, 8, width=16, depth=2, activation='relu', output_activation='identity')
+    fresh.load_state_dict(moe.state_dict())
+    assert torch.equal(fresh.balance_bias, moe.balance_bias)
+    with pytest.raises(ValueError):
+        fresh.forward_mode = 'softmax_topk'
+        fresh.gate(x)
 
 
 def test_norm_modules_off_the_gpu():
@@ -179,12 +186,12 @@ def test_c_entry_points_refuse_before_anything_is_launched():
     lib = abi.load()
     p = 4096
 
-    def norm(n=4, d=8, dtype=abi.BF16, param=abi.BF16, eps=1e-5, x=p, out=p, residual=None, weight=None, mean=None):
+    def norm(n=4, d=8, dtype=abi.BF16, param=abi.BF16, eps=1e-5, x=p, out=p, residual=None, weight=None, mean=None, total=None):
         sh = abi.NormShape(n, d, dtype, param, eps)
-        return lib.d2dmoe_layer_norm(ctypes.byref(sh), x, residual, weight, None, None, out, mean, None, None)
+        return lib.d2dmoe_layer_norm(ctypes.byref(sh), x, residual, weight, None, total, out, mean, None, None)
 
     assert lib.d2dmoe_layer_norm(None, p, None, None, None, None, p, None, None, None) == -1
-    assert norm(x=None) == -1 and norm(out=None) == -1
+    assert norm(x=None) == norm(out=None) == norm(total=p) == -1
     assert norm(n=-1) == -2 and norm(d=0) == -2 and norm(d=(1 << 24) + 1) == -2 and norm(n=1 << 62) == -2
     assert norm(dtype=7) == -3 and norm(param=abi.F16) == -3 and norm(dtype=abi.F32, param=abi.BF16) == -3
     assert norm(eps=-1.0) == norm(eps=math.nan) == norm(eps=math.inf) == abi.E_VALUE
@@ -231,6 +238,36 @@ def test_c_entry_points_refuse_before_anything_is_launched():
     assert grad(k=9) == -2 and grad(scoring=4) == abi.E_VALUE
     assert grad(gr=p + 2) == grad(gw=p + 2) == grad(out=p + 1) == -7
     assert grad(n=0) == 0
+
+
+def test_a_call_runs_on_its_tensors_device(monkeypatch):
+    """The current device is another one than the tensors': the call switches to theirs and takes that device's stream."""
+    from d2dmoe_amd import ops
+    seen = []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            seen.append(('enter', self.dev))
+
+        def __exit__(self, *_):
+            seen.append(('leave', self.dev))
+
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    monkeypatch.setattr(torch.cuda, 'device', Device)
+    monkeypatch.setattr(ops, '_raw_stream', lambda index: 1000 + index)
+
+    def call(*args):
+        seen.append(args)
+        return 0
+
+    ops._launch(torch.device('cuda', 3), call, 'call', 7)
+    assert seen == [('enter', torch.device('cuda', 3)), (7, 1003), ('leave', torch.device('cuda', 3))]
+    seen.clear()
+    ops._launch(torch.device('cuda', 0), call, 'call', 7)
+    assert seen == [(7, 1000)]
 
 
 def test_tensor_level_refusals():

@@ -21,7 +21,8 @@ DEV = 'cuda:0'
 U = 2.0 ** -24
 TINY = 2.0 ** -25
 SHAPES = [(1, 1), (2, 2), (5, 3), (3, 7), (4, 8), (5, 64), (17, 253), (2, 1001), (67, 768), (300, 1280), (33, 2048), (21, 2056), (9, 4096),
-          (5, 4100), (3, 8200), (2, 16384), (2, 20001), (1, 70000), (1030, 96), (4099, 40)]
+          (5, 4100), (3, 8200), (2, 16384), (2, 20001), (1, 70000), (1030, 96), (4099, 40), (71, 65), (333, 121),
+          (129, 128), (77, 200), (1500, 256), (3, 30000)]
 TYPES = [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
          (torch.float16, torch.float16), (torch.float16, torch.float32)]
 
