@@ -43,9 +43,9 @@ __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 // =====================================================================================================
 // Teams: L lanes per token, 64 / L tokens per wave, V consecutive experts per lane (L V >= E, L >= k).
 //
-// A row is read once, as one or two 16-byte loads per lane.  Each lane sorts its V keys (choice, then lowest index: 64 bits
-// that compare as unsigned numbers); the k best are then the team's largest list head, taken k times: two maxima over the
-// team (value, then index) in lane-permute instructions, and the winner's list moves up by one.  Place i ends in lane i, which
+// A row is read once, as one or two 16-byte loads per lane.  Each lane sorts its V keys (choice, then lowest index: 32 bits
+// that compare as unsigned numbers, 64 for float32 logits); the k best are then the team's largest list head, taken k times: a
+// maximum over the team in lane-permute instructions, and the winner's list moves up by one.  Place i ends in lane i, which
 // computes its weight; the dense row goes through a zeroed LDS tile of the wave's tokens, so that it leaves as whole 16-byte
 // stores.  Waves share nothing, so there are no barriers.
 //
@@ -77,26 +77,37 @@ __device__ inline uint32_t order_bits(float v) {
 __device__ inline float from_order_bits(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o); }
 
 // A lane's V choices as keys that compare as unsigned numbers, the larger choice first and the lower index first among equal
-// ones: 64 bits (order of a float32, index), or 32 where the choice is a 16-bit logit.
-template <typename T, int V, bool WIDE> struct Keys {
-  static constexpr bool kWide = WIDE;
-  uint32_t hi[V], lo[V];   // narrow: lo alone
-  __device__ __forceinline__ void set(int j, float c, int e) {
-    const uint32_t low = (uint32_t)(2 * MAX_E - e);
-    if constexpr (WIDE) {
-      hi[j] = c > -INFINITY ? order_bits(c) : 0u;
-      lo[j] = c > -INFINITY ? low : 0u;
+// ones; 0 stands for "not to be chosen".
+//   WIDE   a float32 logit: its order-preserving bits and the index, 32 bits each
+//   HALF   a 16-bit logit: the same in 32 bits together, exact
+//   FIXED  a score (plus bias): 22 bits of fixed point over the row's range and the index in 32 bits.  A step is 2^-22 of the
+//          range, an eighth of what float32 scores leave in doubt anyway where the range is one; choices closer than that
+//          doubt and two steps are told apart in float64.
+enum { WIDE, HALF, FIXED };
+constexpr uint32_t kSteps = (1u << 22) - 2;
+
+template <typename T, int V, int KIND> struct Keys {
+  uint32_t hi[V], lo[V];   // (hi: WIDE)
+  __device__ __forceinline__ void set(int j, float c, int e) {           // WIDE, HALF
+    const bool on = c > -INFINITY;
+    if constexpr (KIND == WIDE) {
+      hi[j] = on ? order_bits(c) : 0u;
+      lo[j] = on ? (uint32_t)(MAX_E - e) : 0u;
     } else {
       uint32_t u;                      // the 16 bits of the logit, on top
       if constexpr (Elem<T>::dtype == D2DMOE_F16) u = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)c) << 16;
       else u = __float_as_uint(c);
       const uint32_t o = (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) & 0xffff0000u;
-      lo[j] = c > -INFINITY ? (o | low) : 0u;
+      lo[j] = on ? (o | (uint32_t)(MAX_E - e)) : 0u;
     }
+  }
+  __device__ __forceinline__ void set_fixed(int j, float c, int e, float least, float scale) {
+    const uint32_t q = 1u + (uint32_t)fminf((c - least) * scale, (float)kSteps);
+    lo[j] = c > -INFINITY ? (q << 10 | (uint32_t)(MAX_E - 1 - e)) : 0u;
   }
   __device__ __forceinline__ void order(int i, int k) {   // larger key to place i
     const uint32_t al = lo[i], bl = lo[k];
-    if constexpr (WIDE) {
+    if constexpr (KIND == WIDE) {
       const uint32_t ah = hi[i], bh = hi[k];
       const bool swap = ((uint64_t)bh << 32 | bl) > ((uint64_t)ah << 32 | al);
       const uint32_t ch = swap ? bh : ah, dh = swap ? ah : bh, cl = swap ? bl : al, dl = swap ? al : bl;
@@ -117,11 +128,12 @@ template <typename T, int V, bool WIDE> struct Keys {
           for (int i = 0; i < (b < V - j - b ? b : V - j - b); ++i)
             if ((i + j) / (2 * a) == (i + j + b) / (2 * a)) order(i + j, i + j + b);
   }
-  // The team's largest key, which leaves its lane's list.  Wide: h is its choice, and `won` the lane it was in -- the lowest of
+  // The team's largest key, which leaves its lane's list.  WIDE: h is its choice, and `won` the lane it was in -- the lowest of
   // those whose list starts with that choice, and so with the lowest index -- found in scalar instructions: the lowest bit
-  // of each L-bit field of the ballot (no field is empty, so the subtraction does not borrow from the next).
+  // of each L-bit field of the ballot (no field is empty, so the subtraction does not borrow from the next); l is the lane's
+  // own head.  Otherwise l is the whole key.
   template <int L> __device__ __forceinline__ void take(uint32_t& h, uint32_t& l, bool& won) {
-    if constexpr (WIDE) {
+    if constexpr (KIND == WIDE) {
       constexpr uint64_t ones = L == 4 ? 0x1111111111111111ull : L == 8 ? 0x0101010101010101ull : L == 16 ? 0x0001000100010001ull
                                                                       : L == 32 ? 0x0000000100000001ull : 1ull;
       h = team_max_u<L>(hi[0]);
@@ -136,15 +148,17 @@ template <typename T, int V, bool WIDE> struct Keys {
     for (int j = 0; j < V; ++j) {      // (values, not places, to choose from: the lists stay in registers)
       const uint32_t lc = lo[j], ln = j + 1 < V ? lo[j + 1 < V ? j + 1 : j] : 0u;
       lo[j] = won ? ln : lc;
-      if constexpr (WIDE) {
+      if constexpr (KIND == WIDE) {
         const uint32_t hc = hi[j], hn = j + 1 < V ? hi[j + 1 < V ? j + 1 : j] : 0u;
         hi[j] = won ? hn : hc;
       }
     }
   }
-  static __device__ __forceinline__ int expert(uint32_t l) { return 2 * MAX_E - (int)(WIDE ? l : (l & 0xffffu)); }
-  static __device__ __forceinline__ float choice(uint32_t h) {
-    if constexpr (WIDE) {
+  static __device__ __forceinline__ int expert(uint32_t l) {
+    return KIND == FIXED ? MAX_E - 1 - (int)(l & 1023u) : MAX_E - (int)(KIND == WIDE ? l : (l & 0xffffu));
+  }
+  static __device__ __forceinline__ float logit(uint32_t h) {            // WIDE, HALF
+    if constexpr (KIND == WIDE) {
       return from_order_bits(h);
     } else {
       const uint32_t o = h >> 16;
@@ -391,9 +405,9 @@ __device__ __forceinline__ int choose_exactly(const float (&z)[V], bool row_bad,
   return place;
 }
 
-// What the choice goes by, each an instance of its own: the logits (no score, no doubt, 32-bit keys for 16-bit types), scores
-// with a bias, or either of them within groups.
-enum { BY_LOGIT, BY_SCORE, IN_GROUPS };
+// What the choice goes by, each an instance of its own: the logits (no score, no doubt), or scores (with a bias, or with sums
+// of them for the groups); among all experts, or within groups.
+enum { BY_LOGIT = 0, BY_SCORE = 1, IN_GROUPS = 2 };
 
 template <typename T, int V, int L, int MODE>
 __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restrict__ logits, T* __restrict__ routing, const RouteArgs A,
@@ -405,7 +419,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
   char* lds = lds_raw + wave * wave_lds;
   if (A.counts != nullptr && blockIdx.x == 0)                 // (filled by the pass over the indices behind this launch)
     for (int e = threadIdx.x; e < A.E; e += WAVES * 64) A.counts[e] = 0;
-  const bool direct = MODE == BY_LOGIT || (MODE == IN_GROUPS && A.bias == nullptr && !A.top2);
+  constexpr bool direct = !(MODE & BY_SCORE), groups = (MODE & IN_GROUPS) != 0;
   const int have = A.E - e0;                                  // experts from e0 on (<= 0: an idle lane)
   const int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
   if (tile * TOK < A.N) {
@@ -457,57 +471,71 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
 #pragma unroll
     for (int j = 0; j < V; ++j) by[j] = bad ? -INFINITY : by[j];
     bool doubt = false;
-    if constexpr (MODE == IN_GROUPS)
+    if constexpr (groups)
       doubt = keep_groups<V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
-    using K = Keys<T, V, MODE != BY_LOGIT || sizeof(T) == 4>;
+    using K = Keys<T, V, !direct ? FIXED : (sizeof(T) == 4 ? WIDE : HALF)>;
     K keys;
+    float near_by = 0.f;                                      // FIXED: the doubt in steps
+    if constexpr (direct) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
+      for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
+    } else {
+      float most = -INFINITY, least = INFINITY;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        most = fmaxf(most, by[j]);
+        least = fminf(least, by[j] > -INFINITY ? by[j] : INFINITY);
+      }
+      most = team_max<L>(most);
+      least = -team_max<L>(-least);
+      const float range = most - least;
+      if (most > -INFINITY && !finite(range)) doubt = true;   // (a bias of +inf, or two of opposite ends of the type)
+      const float scale = fminf((float)kSteps * __builtin_amdgcn_rcpf(fmaxf(range, 0x1p-80f)), 0x1p100f);
+      near_by = (0x1p-19f + 0x1p-22f * fmaxf(fabsf(most), fabsf(least))) * scale + 2.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) keys.set_fixed(j, by[j], e0 + j, least, scale);
+    }
     keys.sort();
     uint32_t mine_hi = 0, mine_lo = 0;                        // place tl's key
     uint32_t hi, lo;
     bool won;
+    constexpr bool wide = direct && sizeof(T) == 4;
     uint32_t* places = (uint32_t*)lds + team * A.K;           // wide keys: the winner's lane leaves its index here
-    if constexpr (K::kWide) wave_sync();
+    if constexpr (wide) wave_sync();
     for (int i = 0; i < A.K; ++i) {
       keys.template take<L>(hi, lo, won);
-      if constexpr (K::kWide) {
+      if constexpr (wide) {
         if (won) places[i] = lo;
         mine_hi = tl == i ? hi : mine_hi;
       } else {
         mine_lo = tl == i ? lo : mine_lo;
       }
     }
-    if constexpr (K::kWide) {
+    if constexpr (wide) {
       wave_sync();
       if (tl < A.K) mine_lo = places[tl];
     } else {
       mine_hi = mine_lo;
     }
-    if (MODE != BY_LOGIT && !direct) {
+    int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
+    float zi = -INFINITY;
+    if constexpr (direct) {
+      if (at >= 0) zi = K::logit(mine_hi);
+    } else {
       // places next to each other, and the last one with the first that was left out
       keys.template take<L>(hi, lo, won);
-      const uint32_t next = tl == A.K - 1 ? hi : (uint32_t)__shfl_down((int)mine_hi, 1, kWave);
-      const float c = K::choice(mine_hi), d = K::choice(next);
-      if (tl < A.K && next != 0 && c - d <= 0x1p-19f + 0x1p-22f * fabsf(c)) doubt = true;
-    }
-    int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
-    if constexpr (MODE != BY_LOGIT) {
-      if (!direct && __ballot(doubt) != 0ull) at = choose_exactly<V, L, MODE == IN_GROUPS>(z, bad, A, (double*)lds);
-    }
-    // place tl's weight
-    float zi = -INFINITY;
-    if (MODE == BY_LOGIT) {
-      if (at >= 0) zi = K::choice(mine_hi);
-    } else {
+      const uint32_t next = tl == A.K - 1 ? lo : (uint32_t)__shfl_down((int)mine_lo, 1, kWave);
+      if (tl < A.K && next != 0 && (float)((mine_lo >> 10) - (next >> 10)) <= near_by) doubt = true;
+      if (__ballot(doubt) != 0ull) at = choose_exactly<V, L, groups>(z, bad, A, (double*)lds);
       // the chosen logits come out of the lanes that hold them through LDS
       float* zs = (float*)lds + team * (L * V);
       wave_sync();
 #pragma unroll
-      for (int j = 0; j < V; j += 4) *(float4*)(zs + e0 + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+      for (int j = 0; j < V; ++j) zs[e0 + j] = z[j];
       wave_sync();
       if (at >= 0) zi = zs[at];
     }
+    // place tl's weight
     float ref = A.softmax ? top : 0.f;
     if (A.renorm) {
       ref = team_max<L>(A.softmax ? zi : fminf(zi, 0.f));
@@ -898,8 +926,9 @@ hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, 
   if (A.G > 1) wave += tok * A.G * (sizeof(double) + 1);
   wave = (wave + 15) / 16 * 16;
   const size_t lds = WAVES * wave;
-  const auto kern = A.G > 1 ? route_team_kernel<T, V, L, IN_GROUPS>
-                            : (A.bias ? route_team_kernel<T, V, L, BY_SCORE> : route_team_kernel<T, V, L, BY_LOGIT>);
+  const bool score = A.bias || (A.G > 1 && A.top2);
+  const auto kern = A.G > 1 ? (score ? route_team_kernel<T, V, L, BY_SCORE | IN_GROUPS> : route_team_kernel<T, V, L, BY_LOGIT | IN_GROUPS>)
+                            : (score ? route_team_kernel<T, V, L, BY_SCORE> : route_team_kernel<T, V, L, BY_LOGIT>);
   if (lds > (64u << 10)) {   // (E near 1024 with hundreds of groups)
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
@@ -907,6 +936,7 @@ hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, 
   constexpr int64_t tokens = SLICE * WAVES * (64 / L);
   for (int64_t done = 0; done < A.N; done += tokens) {
     RouteArgs part = A;
+    part.inv_lanes = (float)V * A.inv_size;
     part.N = A.N - done < tokens ? A.N - done : tokens;
     if (A.indices) part.indices += done * A.K;
     if (A.weights) part.weights += done * A.K;
@@ -925,10 +955,12 @@ hipError_t forward_t(const d2dmoe_route_shape& sh, const void* logits, const flo
   if (sh.k <= 64) {
     const RouteArgs A{bias, indices, weights, counts, sh.n_tokens, sh.n_experts, sh.k, softmax, sh.n_groups, sh.kept_groups, top2,
                       sh.renormalise, sh.scale, sh.n_experts / sh.n_groups, (float)sh.n_groups / (float)sh.n_experts,
-                      1.f / (float)sh.n_groups, (sh.n_experts > 512 ? 16.f : 8.f) * (float)sh.n_groups / (float)sh.n_experts};
+                      1.f / (float)sh.n_groups, 0.f};
     const T* z = (const T*)logits;
     T* r = (T*)routing;
     if (sh.n_experts > 512) return forward_l<T, 16, 64>(sh, z, r, A, s);
+    if (sh.n_experts <= 16 && sh.k <= 4)   // (fewer experts per lane: 2^20 rows of 8 are 33 MB and 31 us at eight per lane)
+      return sh.n_experts <= 8 ? forward_l<T, 2, 4>(sh, z, r, A, s) : forward_l<T, 4, 4>(sh, z, r, A, s);
     switch (team_lanes(sh.n_experts, 8, sh.k)) {
       case 4: return forward_l<T, 8, 4>(sh, z, r, A, s);
       case 8: return forward_l<T, 8, 8>(sh, z, r, A, s);

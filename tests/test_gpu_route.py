@@ -70,7 +70,7 @@ def _check_grad(z, idx, q, scoring, renormalise, scale, t, grad, tol):
     assert grad.dtype == t and (err <= bound + _half(t) * np.abs(want) + 2.0 ** -25 * (t == torch.float16)).all(), (err - bound).max()
 
 
-EXPERTS = [1, 2, 3, 7, 8, 24, 60, 64, 65, 100, 128, 129, 160, 256, 320, 512, 513, 1000, 1024]
+EXPERTS = [1, 2, 3, 7, 8, 13, 16, 24, 60, 64, 65, 100, 128, 129, 160, 256, 320, 512, 513, 1000, 1024]
 
 
 @pytest.mark.parametrize('t', [torch.float32, torch.bfloat16, torch.float16])
@@ -98,7 +98,7 @@ def test_plain_choice(e, t):
 
 
 @pytest.mark.parametrize('t', [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize('e,groups,kept,k', [(8, 2, 1, 3), (8, 4, 2, 4), (8, 8, 3, 2), (12, 3, 2, 5), (24, 3, 1, 8), (60, 5, 2, 6), (64, 8, 4, 8),
+@pytest.mark.parametrize('e,groups,kept,k', [(4, 2, 1, 2), (8, 4, 3, 2), (12, 3, 2, 4), (16, 2, 1, 4), (16, 8, 3, 2), (8, 2, 1, 3), (8, 4, 2, 4), (8, 8, 3, 2), (12, 3, 2, 5), (24, 3, 1, 8), (60, 5, 2, 6), (64, 8, 4, 8),
                                              (96, 8, 3, 6), (128, 4, 2, 8), (128, 64, 9, 8), (160, 8, 3, 6), (256, 8, 4, 8), (256, 1, 1, 8),
                                              (320, 10, 5, 8), (512, 2, 1, 4), (512, 16, 4, 12), (1000, 10, 4, 8), (1024, 32, 4, 8),
                                              (1024, 1024, 40, 33)])
