@@ -378,17 +378,37 @@ def forward(x: torch.Tensor, router_w1: Optional[torch.Tensor], router_w2: Optio
 
 
 # ---- layer norm and routing by scores --------------------------------------------------------------------------------
-# the handle of a device's current stream (torch.cuda.current_stream builds a Stream object around it: 2.7 us of a 12 us call)
+# The handle of a device's current stream: torch.cuda.current_stream builds a Stream object around it, 2.7 us of a 12 us call.
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _launch(dev: torch.device, fn, what: str, *args) -> None:
+def _gpu_index(*tensors: Optional[torch.Tensor]) -> int:
+    """_require_gpu for calls of a few microseconds: the index of the one device that all tensors are on."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        i = t.get_device()       # -1 off the GPU
+        if i != index:
+            if i < 0:
+                raise abi.D2DMoEError('the HIP path needs tensors on a ROCm device; there is no CPU fallback')
+            if index >= 0:
+                raise abi.D2DMoEError('all tensors must live on the same device')
+            index = i
+        if not t.is_contiguous():
+            raise abi.D2DMoEError('the HIP path needs contiguous tensors')
+    if index < 0:
+        raise abi.D2DMoEError('the HIP path needs tensors on a ROCm device; there is no CPU fallback')
+    return index
+
+
+def _launch(index: int, fn, what: str, *args) -> None:
     """One library call on the tensors' device and that device's current stream."""
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(dev.index))
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev.index))
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
     if status != 0:
         abi.check(status, what)
 
@@ -418,7 +438,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise abi.D2DMoEError(f'layer_norm: residual is {residual.dtype} {tuple(residual.shape)}, x is {x.dtype} {tuple(x.shape)}')
     if x.dim() != 2:
         raise abi.D2DMoEError(f'layer_norm: x has {x.dim()} dimensions, the rows come as [N,D]')
-    dev = _require_gpu(x, residual, weight, bias)
+    index = _gpu_index(x, residual, weight, bias)
     lib = abi.load()
     n, d = x.shape
     pcode = _norm_params('layer_norm', d, x.dtype, weight, bias)
@@ -426,9 +446,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     total = None if residual is None else torch.empty_like(x)
     mean = rstd = None
     if want_stats:
-        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=dev).unbind(0)
+        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=x.device).unbind(0)
     sh = abi.NormShape(n, d, code, pcode, eps)
-    _launch(dev, lib.d2dmoe_layer_norm, 'd2dmoe_layer_norm', ctypes.byref(sh), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
+    _launch(index, lib.d2dmoe_layer_norm, 'd2dmoe_layer_norm', ctypes.byref(sh), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
             _ptr(total), out.data_ptr(), _ptr(mean), _ptr(rstd))
     return out, total, mean, rstd
 
@@ -450,7 +470,8 @@ def layer_norm_backward(grad_out: torch.Tensor, h: torch.Tensor, weight: Optiona
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.dtype != torch.float32 or t.shape != (n,):
             raise abi.D2DMoEError(f'layer_norm_backward: {name} is {t.dtype} {tuple(t.shape)}, expected float32 ({n},)')
-    dev = _require_gpu(h, grad_out, grad_sum, weight, mean, rstd)
+    index = _gpu_index(h, grad_out, grad_sum, weight, mean, rstd)
+    dev = h.device
     lib = abi.load()
     pcode = _norm_params('layer_norm_backward', d, h.dtype, weight)
     ptype = weight.dtype if weight is not None else (param_dtype or h.dtype)
@@ -469,7 +490,7 @@ def layer_norm_backward(grad_out: torch.Tensor, h: torch.Tensor, weight: Optiona
         # (a buffer of this call's own, not the one kept per stream: a captured call keeps its buffer with its graph)
         nbytes = lib.d2dmoe_layer_norm_workspace_bytes(ctypes.byref(sh))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, lib.d2dmoe_layer_norm_backward, 'd2dmoe_layer_norm_backward', ctypes.byref(sh), grad_out.data_ptr(), _ptr(grad_sum),
+    _launch(index, lib.d2dmoe_layer_norm_backward, 'd2dmoe_layer_norm_backward', ctypes.byref(sh), grad_out.data_ptr(), _ptr(grad_sum),
             h.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(grad), _ptr(gw), _ptr(gb), _ptr(ws), nbytes)
     return grad, gw, gb
 
@@ -498,13 +519,14 @@ def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bi
         raise abi.D2DMoEError(f'route_topk: k = {k} of {e} experts')
     if choice_bias is not None and (choice_bias.dtype != torch.float32 or choice_bias.shape != (e,)):
         raise abi.D2DMoEError(f'route_topk: choice_bias is {choice_bias.dtype} {tuple(choice_bias.shape)}, expected float32 ({e},)')
-    dev = _require_gpu(logits, choice_bias)
+    index = _gpu_index(logits, choice_bias)
+    dev = logits.device
     lib = abi.load()
     routing = torch.empty_like(logits)
     indices = torch.empty(n, k, dtype=torch.int32, device=dev)
     weights = torch.empty(n, k, dtype=torch.float32, device=dev)
     counts = torch.empty(e, dtype=torch.int32, device=dev) if want_counts else None
-    _launch(dev, lib.d2dmoe_route_topk, 'd2dmoe_route_topk', ctypes.byref(sh), logits.data_ptr(), _ptr(choice_bias),
+    _launch(index, lib.d2dmoe_route_topk, 'd2dmoe_route_topk', ctypes.byref(sh), logits.data_ptr(), _ptr(choice_bias),
             routing.data_ptr(), indices.data_ptr(), weights.data_ptr(), _ptr(counts))
     return routing, indices, weights, counts
 
@@ -525,9 +547,9 @@ def route_topk_backward(logits: torch.Tensor, indices: torch.Tensor, scoring: st
     if grad_weights is not None and (grad_weights.dtype != torch.float32 or grad_weights.shape != indices.shape):
         raise abi.D2DMoEError(f'route_topk_backward: grad_weights is {grad_weights.dtype} {tuple(grad_weights.shape)}, expected float32 '
                               f'{tuple(indices.shape)}')
-    dev = _require_gpu(logits, indices, grad_routing, grad_weights)
+    index = _gpu_index(logits, indices, grad_routing, grad_weights)
     lib = abi.load()
     grad = torch.empty_like(logits)
-    _launch(dev, lib.d2dmoe_route_topk_backward, 'd2dmoe_route_topk_backward', ctypes.byref(sh), logits.data_ptr(), indices.data_ptr(),
+    _launch(index, lib.d2dmoe_route_topk_backward, 'd2dmoe_route_topk_backward', ctypes.byref(sh), logits.data_ptr(), indices.data_ptr(),
             _ptr(grad_routing), _ptr(grad_weights), grad.data_ptr())
     return grad

@@ -263,10 +263,10 @@ def test_a_call_runs_on_its_tensors_device(monkeypatch):
         seen.append(args)
         return 0
 
-    ops._launch(torch.device('cuda', 3), call, 'call', 7)
-    assert seen == [('enter', torch.device('cuda', 3)), (7, 1003), ('leave', torch.device('cuda', 3))]
+    ops._launch(3, call, 'call', 7)
+    assert seen == [('enter', 3), (7, 1003), ('leave', 3)]
     seen.clear()
-    ops._launch(torch.device('cuda', 0), call, 'call', 7)
+    ops._launch(0, call, 'call', 7)
     assert seen == [(7, 1000)]
 
 
