@@ -266,18 +266,18 @@ __device__ __forceinline__ void score_groups(const C* tile, C* score, const Rout
   }
 }
 
-// Drops the groups that do not stay from by[] (-inf); returns whether a group's place was in doubt.  tile: T E values, score:
-// T G values of the wave's own LDS.
-template <int V, int L>
-__device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, float near_abs, float near_rel, float* tile, float* score) {
+// Drops the groups that do not stay from by[] (-inf); returns whether a group's place was in doubt (NEAR).  tile: T E values,
+// score: T G values of the wave's own LDS.
+template <bool NEAR, int V, int L, typename C>
+__device__ __forceinline__ bool keep_groups(C (&by)[V], const RouteArgs& A, C near_abs, C near_rel, C* tile, C* score) {
   constexpr int T = 64 / L;
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L;
   const int size = A.size, G = A.G, e0 = tl * V;
-  const float low = -INFINITY;
+  const C low = -(C)INFINITY;
   wave_sync();
   if (size % V == 0) {
     // whole lanes per group: the two largest of ever longer runs of lanes, up to the group's end, in its first lane
-    float a = low, b = low;
+    C a = low, b = low;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       b = larger(b, smaller(a, by[j]));
@@ -285,7 +285,7 @@ __device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, 
     }
     const int lanes = size / V, of = small_div(tl, A.inv_lanes), pos = tl - of * lanes;
     for (int off = 1; off < lanes; off <<= 1) {
-      const float oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
+      const C oa = __shfl_down(a, off, kWave), ob = __shfl_down(b, off, kWave);
       if (pos + off < lanes) {
         b = larger(larger(b, ob), smaller(a, oa));
         a = larger(a, oa);
@@ -297,12 +297,11 @@ __device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, 
     for (int j = 0; j < V; ++j)
       if (e0 + j < A.E) tile[team * A.E + e0 + j] = by[j];
     wave_sync();
-    score_groups<float, T>(tile, score, A);
+    score_groups<C, T>(tile, score, A);
   }
   wave_sync();
   uint8_t* stays = (uint8_t*)tile;
-  const bool doubt = near_abs > 0.f ? rank_groups<float, T, true>(score, stays, A, near_abs, near_rel)
-                                    : rank_groups<float, T, false>(score, stays, A, 0.f, 0.f);
+  const bool doubt = rank_groups<C, T, NEAR>(score, stays, A, near_abs, near_rel);
   wave_sync();
   int g = small_div(e0, A.inv_size);
   if (size % V == 0) {
@@ -324,7 +323,7 @@ __device__ __forceinline__ bool keep_groups(float (&by)[V], const RouteArgs& A, 
 // The choice on float64 scores: returns place tl's expert (or -1).  Few waves come here, but a launch waits for its last one,
 // and the kernel's occupancy is set by its widest part.  So: one exponential at a time (eight interleaved take 100 registers),
 // from LDS to LDS, then the choices in registers and the maxima over the team by lane permutes, as in the float32 choice.
-// tiles[]: T rows of E, T rows of G scores, T G flags.
+// tiles[]: T rows of E, T rows of G scores.
 template <int V, int L, bool GROUPS>
 __device__ __forceinline__ int choose_exactly(const float (&z)[V], bool row_bad, const RouteArgs& A, double* tiles) {
   constexpr int TOK = 64 / L;
@@ -360,22 +359,7 @@ __device__ __forceinline__ int choose_exactly(const float (&z)[V], bool row_bad,
     if (A.bias != nullptr) c += (double)b[j];
     by[j] = (z[j] == -INFINITY || row_bad) ? low : c + 0.0;
   }
-  if constexpr (GROUPS) {
-    double* score = tiles + TOK * A.E;
-    uint8_t* stays = (uint8_t*)(score + TOK * A.G);
-    wave_sync();
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j < A.E) tile[e0 + j] = by[j];
-    wave_sync();
-    score_groups<double, TOK>(tiles, score, A);
-    wave_sync();
-    rank_groups<double, TOK, false>(score, stays, A, 0.0, 0.0);
-    wave_sync();
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j < A.E && !stays[team * A.G + small_div(e0 + j, A.inv_size)]) by[j] = low;
-  }
+  if constexpr (GROUPS) keep_groups<false, V, L>(by, A, 0.0, 0.0, tiles, tiles + TOK * A.E);
   int place = -1;
 #pragma unroll 1
   for (int i = 0; i < A.K; ++i) {
@@ -472,7 +456,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     for (int j = 0; j < V; ++j) by[j] = bad ? -INFINITY : by[j];
     bool doubt = false;
     if constexpr (groups)
-      doubt = keep_groups<V, L>(by, A, direct ? 0.f : 0x1p-18f, direct ? 0.f : 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
+      doubt = keep_groups<!direct, V, L>(by, A, 0x1p-18f, 0x1p-21f, (float*)lds, (float*)lds + TOK * A.E);
     using K = Keys<T, V, !direct ? FIXED : (sizeof(T) == 4 ? WIDE : HALF)>;
     K keys;
     float near_by = 0.f;                                      // FIXED: the doubt in steps
@@ -919,20 +903,16 @@ inline int64_t team_blocks(int64_t N, int L) { return cdiv64(cdiv64(N, 64 / L), 
 
 template <typename T, int V, int L>
 hipError_t forward_l(const d2dmoe_route_shape& sh, const T* logits, T* routing, const RouteArgs& A, hipStream_t s) {
-  // per wave: the dense tile; with scores the exact choice's T E values, and the chosen logits; with groups also T G scores and flags
+  // per wave: the dense tile; with scores the exact choice's T E values, and the chosen logits; with groups also T G scores
   const size_t tok = 64 / L;
   size_t wave = tok * A.E * sizeof(T);
   if (A.G > 1 || A.bias) wave = tok * A.E * sizeof(double) > 64 * V * sizeof(float) ? tok * A.E * sizeof(double) : 64 * V * sizeof(float);
-  if (A.G > 1) wave += tok * A.G * (sizeof(double) + 1);
+  if (A.G > 1) wave += tok * A.G * sizeof(double);
   wave = (wave + 15) / 16 * 16;
-  const size_t lds = WAVES * wave;
+  const size_t lds = WAVES * wave;                            // (64 KB at the most: tok E <= 64 V, G <= E)
   const bool score = A.bias || (A.G > 1 && A.top2);
   const auto kern = A.G > 1 ? (score ? route_team_kernel<T, V, L, BY_SCORE | IN_GROUPS> : route_team_kernel<T, V, L, BY_LOGIT | IN_GROUPS>)
                             : (score ? route_team_kernel<T, V, L, BY_SCORE> : route_team_kernel<T, V, L, BY_LOGIT>);
-  if (lds > (64u << 10)) {   // (E near 1024 with hundreds of groups)
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
   constexpr int64_t tokens = SLICE * WAVES * (64 / L);
   for (int64_t done = 0; done < A.N; done += tokens) {
     RouteArgs part = A;
