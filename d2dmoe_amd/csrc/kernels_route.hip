@@ -54,12 +54,12 @@ __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 // other score of a pair shares; sigmoid: 4.2 u) and its sum with a bias by u |c| more.  Where two choices whose order matters
 // lie within 2^-19 + 2^-22 |c| of each other (sums of two scores: twice that) -- places next to one another in the list, the
 // last place and the first one left out, a group that stays and one that goes -- the wave repeats its choice on float64
-// scores; a row or two in a thousand do.  Their waves finish last: 16384 x 256 takes 17 us with a bias, 13 us with one that
-// leaves nothing in doubt, 29 us with one (all zeros, 16-bit logits) that leaves every wave in doubt.
+// scores; a row or two in a thousand do.  Their waves finish last: 16384 x 256 takes 16.6 us with a bias, 12 us with one that
+// leaves nothing in doubt, 30 us with one (all zeros, 16-bit logits) that leaves every wave in doubt.
 //
-// Bound by vector instructions, not by memory: 390 per wave of four tokens at 128 experts and 8 places in bf16, 860 per wave
+// Bound by vector instructions, not by memory: 388 per wave of four tokens at 128 experts and 8 places in bf16, 776 per wave
 // of two at 256 in float32 with groups and a bias.  50432 x 128 bf16: 11 us (29 MB: 5.6 us at this card's copy rate);
-// 16384 x 256 float32 in groups: 22 us (35 MB: 6.7 us).  Before: one wave per token with float64 throughout, 396 and 206 us.
+// 16384 x 256 float32 in groups: 20 us (35 MB: 6.7 us), 131072 x 256: 85 us.  Before: one wave per token with float64 throughout, 396 and 206 us.
 // =====================================================================================================
 constexpr int WAVES = 4;   // per workgroup
 
@@ -80,11 +80,14 @@ __device__ inline float from_order_bits(uint32_t o) { return __uint_as_float((o 
 // ones; 0 stands for "not to be chosen".
 //   WIDE   a float32 logit: its order-preserving bits and the index, 32 bits each
 //   HALF   a 16-bit logit: the same in 32 bits together, exact
-//   FIXED  a score (plus bias): 22 bits of fixed point over the row's range and the index in 32 bits.  A step is 2^-22 of the
-//          range, an eighth of what float32 scores leave in doubt anyway where the range is one; choices closer than that
-//          doubt and two steps are told apart in float64.
+//   FIXED  a score (plus bias): 22 bits of fixed point over the row's range and the index in 32 bits; below kNone (a zero in
+//          those bits) it stands for "not to be chosen".  A step is 2^-22 of the range, an eighth of what float32 scores leave
+//          in doubt anyway where the range is one; choices closer than that doubt and two steps are told apart in float64.
+//          The range's ends keep a margin, since the multiplication and addition that makes a step number shares one rounding
+//          error of up to a quarter of the doubt among the row's numbers: a doubt of kMargin steps goes to float64 as a whole.
 enum { WIDE, HALF, FIXED };
-constexpr uint32_t kSteps = (1u << 22) - 2;
+constexpr float kTop = (1 << 22) - 1, kMargin = 1 << 15;
+constexpr uint32_t kNone = MAX_E;
 
 template <typename T, int V, int KIND> struct Keys {
   uint32_t hi[V], lo[V];   // (hi: WIDE)
@@ -101,9 +104,8 @@ template <typename T, int V, int KIND> struct Keys {
       lo[j] = on ? (o | (uint32_t)(MAX_E - e)) : 0u;
     }
   }
-  __device__ __forceinline__ void set_fixed(int j, float c, int e, float least, float scale) {
-    const uint32_t q = 1u + (uint32_t)fminf((c - least) * scale, (float)kSteps);
-    lo[j] = c > -INFINITY ? (q << 10 | (uint32_t)(MAX_E - 1 - e)) : 0u;
+  __device__ __forceinline__ void set_fixed(int j, float c, int e, float scale, float offset) {   // (-inf and NaN: 0)
+    lo[j] = (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c, scale, offset), 0.f, kTop) << 10 | (uint32_t)(MAX_E - 1 - e);
   }
   __device__ __forceinline__ void order(int i, int k) {   // larger key to place i
     const uint32_t al = lo[i], bl = lo[k];
@@ -170,9 +172,9 @@ template <typename T, int V, int KIND> struct Keys {
   }
 };
 
-__device__ inline float larger(float a, float b) { return fmaxf(a, b); }
+__device__ inline float larger(float a, float b) { return max1(a, b); }
 __device__ inline double larger(double a, double b) { return fmax(a, b); }
-__device__ inline float smaller(float a, float b) { return fminf(a, b); }
+__device__ inline float smaller(float a, float b) { return min1(a, b); }
 __device__ inline double smaller(double a, double b) { return fmin(a, b); }
 
 // V consecutive elements from any address; those at `count` and beyond read as `fill`
@@ -250,6 +252,12 @@ __device__ __forceinline__ bool rank_groups(const C* score, uint8_t* stays, cons
   return __ballot(doubt) != 0ull;
 }
 
+// A group's score from its two largest choices.  (Two of float32's lowest value, as masks use it, overflow: more than none still.)
+__device__ inline float add_best(float a, float b) { return max1(a + b, -0x1.fffffep127f); }
+__device__ inline double add_best(double a, double b) { return a + b; }
+template <typename C>
+__device__ __forceinline__ C group_score(const RouteArgs& A, C a, C b) { return (A.top2 && b > -(C)INFINITY) ? add_best(a, b) : a; }
+
 // The scores of the T G groups from the choices in tile[] (T rows of E).
 template <typename C, int T>
 __device__ __forceinline__ void score_groups(const C* tile, C* score, const RouteArgs& A) {
@@ -262,7 +270,7 @@ __device__ __forceinline__ void score_groups(const C* tile, C* score, const Rout
       b = larger(b, smaller(a, v));
       a = larger(a, v);
     }
-    score[p] = (A.top2 && b > low) ? a + b : a;
+    score[p] = group_score(A, a, b);
   }
 }
 
@@ -291,7 +299,7 @@ __device__ __forceinline__ bool keep_groups(C (&by)[V], const RouteArgs& A, C ne
         a = larger(a, oa);
       }
     }
-    if (pos == 0 && e0 < A.E) score[team * G + of] = (A.top2 && b > low) ? a + b : a;
+    if (pos == 0 && e0 < A.E) score[team * G + of] = group_score(A, a, b);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -418,7 +426,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       bad = bad || z[j] != z[j];
-      top = fmaxf(top, z[j]);
+      top = max1(top, z[j]);
     }
     if (A.softmax) bad = bad || top == INFINITY;
     const bool whole = A.softmax && !(A.renorm && direct);    // the row's softmax is needed, not only its order
@@ -467,17 +475,18 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       float most = -INFINITY, least = INFINITY;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        most = fmaxf(most, by[j]);
-        least = fminf(least, by[j] > -INFINITY ? by[j] : INFINITY);
+        most = max1(most, by[j]);
+        least = min1(least, by[j] > -INFINITY ? by[j] : INFINITY);
       }
       most = team_max<L>(most);
       least = -team_max<L>(-least);
-      const float range = most - least;
-      if (most > -INFINITY && !finite(range)) doubt = true;   // (a bias of +inf, or two of opposite ends of the type)
-      const float scale = fminf((float)kSteps * __builtin_amdgcn_rcpf(fmaxf(range, 0x1p-80f)), 0x1p100f);
+      const float range = most - least;                       // (infinite: a scale of 0, and nothing told apart)
+      const float scale = fminf((kTop - 2.f * kMargin) * __builtin_amdgcn_rcpf(fmaxf(range, 0x1p-80f)), 0x1p100f);
+      const float offset = kMargin - least * scale;
       near_by = (0x1p-19f + 0x1p-22f * fmaxf(fabsf(most), fabsf(least))) * scale + 2.f;
+      if (most > -INFINITY && !(near_by < kMargin)) doubt = true;   // (also a NaN: a bias of +inf)
 #pragma unroll
-      for (int j = 0; j < V; ++j) keys.set_fixed(j, by[j], e0 + j, least, scale);
+      for (int j = 0; j < V; ++j) keys.set_fixed(j, by[j], e0 + j, scale, offset);
     }
     keys.sort();
     uint32_t mine_hi = 0, mine_lo = 0;                        // place tl's key
@@ -501,7 +510,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     } else {
       mine_hi = mine_lo;
     }
-    int at = (tl < A.K && mine_hi != 0) ? K::expert(mine_lo) : -1;
+    int at = (tl < A.K && mine_hi >= (direct ? 1u : kNone)) ? K::expert(mine_lo) : -1;
     float zi = -INFINITY;
     if constexpr (direct) {
       if (at >= 0) zi = K::logit(mine_hi);
@@ -509,7 +518,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       // places next to each other, and the last one with the first that was left out
       keys.template take<L>(hi, lo, won);
       const uint32_t next = tl == A.K - 1 ? lo : (uint32_t)__shfl_down((int)mine_lo, 1, kWave);
-      if (tl < A.K && next != 0 && (float)((mine_lo >> 10) - (next >> 10)) <= near_by) doubt = true;
+      if (tl < A.K && next >= kNone && (float)((mine_lo >> 10) - (next >> 10)) <= near_by) doubt = true;
       if (__ballot(doubt) != 0ull) at = choose_exactly<V, L, groups>(z, bad, A, (double*)lds);
       // the chosen logits come out of the lanes that hold them through LDS
       float* zs = (float*)lds + team * (L * V);

@@ -7,8 +7,22 @@
 
 namespace d2dmoe {
 
+// The larger (smaller) of two numbers in one instruction: the middle one of them and an infinity, which the empty asm hides,
+// since the compiler makes fmaxf of it otherwise, and of that up to three instructions (operands made quiet first).  A NaN loses
+// in max1, as in fmaxf; min1 takes none.
+__device__ __forceinline__ float max1(float a, float b) {
+  float end = INFINITY;
+  asm("" : "+s"(end));
+  return __builtin_amdgcn_fmed3f(a, b, end);
+}
+__device__ __forceinline__ float min1(float a, float b) {
+  float end = -INFINITY;
+  asm("" : "+s"(end));
+  return __builtin_amdgcn_fmed3f(a, b, end);
+}
+
 template <int CTRL>
-__device__ inline uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+__device__ inline uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
 
 template <int L, typename Op>
 __device__ inline uint32_t team_reduce(uint32_t v, Op op) {
@@ -30,7 +44,7 @@ template <int L>
 __device__ inline uint32_t team_max_u(uint32_t v) { return team_reduce<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
 template <int L>
 __device__ inline float team_max(float v) {
-  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(max1(__uint_as_float(a), __uint_as_float(b))); }));
 }
 template <int L>
 __device__ inline float team_sum(float v) {

@@ -143,6 +143,27 @@ def test_neighbours_that_float32_scores_do_not_tell_apart(scoring):
     _check(zb[:400], 8, scoring, torch.zeros(64), {}, torch.bfloat16, (got[0][:400], got[1][:400], got[2][:400], None))
 
 
+@pytest.mark.parametrize('e', [4, 8, 16, 64, 200, 1024])
+def test_biases_of_any_size(e):
+    """What the choice goes by spans anything from a float32 step of a large offset to the ends of the type: the choice is still
+    that of the float64 sums."""
+    g = torch.Generator().manual_seed(e)
+    z = _logits(150 if e <= 64 else 20, e, torch.float32, seed=e)
+    lowest, some = torch.finfo(torch.float32).min, torch.rand(e, generator=g)
+    biases = {'offset': torch.full((e,), 1000.0), 'two steps of an offset': 1000.0 + (some > 0.5) * 2.0 ** -13,
+              'far': some * 1e30, 'tiny': some * 1e-30, 'lowest': torch.where(some < 0.7, lowest, 0.0), 'all lowest': torch.full((e,), lowest),
+              'ends': torch.where(some < 0.4, lowest, torch.where(some < 0.6, 3e38, 3.2e38)), 'two low ones': torch.where(some < 0.5, lowest, -3.3e38),
+              'inf': torch.where(some < 0.3, math.inf, 0.0), 'infs': torch.where(some < 0.3, math.inf, torch.where(some < 0.6, -math.inf, lowest)),
+              'none': torch.full((e,), -math.inf), 'one': torch.where(torch.arange(e) == e // 2, 0.0, -math.inf)}
+    for name, bias in biases.items():
+        for scoring in ('softmax', 'sigmoid'):
+            for kw in ({}, dict(n_groups=4, kept_groups=2, group_score='top2'), dict(n_groups=4, kept_groups=2, group_score='max')):
+                k = min(4, e // 2)
+                print('bias', e, name, scoring, kw, flush=True)
+                got = _ops().route_topk(z.to(DEV), k, scoring, bias.to(DEV), want_counts=True, **kw)
+                _check(z, k, scoring, bias, kw, torch.float32, got)
+
+
 def test_scores_that_underflow_still_share_their_weight():
     """Chosen scores of 1e-60 and less: renormalised weights go by their ratio."""
     z = torch.tensor([[-140.0, -139.0, -150.0, -400.0], [-3e38, -3e38, -3e38, -3e38]])
