@@ -517,7 +517,8 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     } else {
       // places next to each other, and the last one with the first that was left out
       keys.template take<L>(hi, lo, won);
-      const uint32_t next = tl == A.K - 1 ? lo : (uint32_t)__shfl_down((int)mine_lo, 1, kWave);
+      const uint32_t after = (uint32_t)__shfl_down((int)mine_lo, 1, kWave);   // (by all lanes: a lane that is switched off gives 0)
+      const uint32_t next = tl == A.K - 1 ? lo : after;
       if (tl < A.K && next >= kNone && (float)((mine_lo >> 10) - (next >> 10)) <= near_by) doubt = true;
       if (__ballot(doubt) != 0ull) at = choose_exactly<V, L, groups>(z, bad, A, (double*)lds);
       // the chosen logits come out of the lanes that hold them through LDS

@@ -143,6 +143,28 @@ def test_neighbours_that_float32_scores_do_not_tell_apart(scoring):
     _check(zb[:400], 8, scoring, torch.zeros(64), {}, torch.bfloat16, (got[0][:400], got[1][:400], got[2][:400], None))
 
 
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('e,k', [(2, 1), (4, 2), (8, 4), (16, 4), (24, 4), (64, 8), (128, 8), (256, 8), (256, 32), (512, 8), (1000, 20), (1024, 64)])
+def test_one_pair_that_float32_scores_do_not_tell_apart(e, k, scoring):
+    """Row p: the choices lie far apart but for places p and p + 1, whose logits are neighbouring float32 numbers, the larger one at
+    the higher index.  Every place has its turn, the last one with the first that is left out among them."""
+    g = torch.Generator().manual_seed(e + k)
+    z = torch.empty(k, e)
+    for p in range(k):
+        falling = 1.0 - torch.arange(e) * 2.0 / e          # by place
+        falling[p] = torch.nextafter(falling[p + 1], torch.tensor(9.0))
+        at = torch.randperm(e, generator=g)
+        if at[p] < at[p + 1]:
+            at[p], at[p + 1] = at[p + 1].clone(), at[p].clone()
+        z[p, at] = falling
+    for groups in (1, 2):
+        kw = dict(n_groups=groups, kept_groups=groups, group_score='top2')
+        got = _ops().route_topk(z.to(DEV), k, scoring, torch.zeros(e, device=DEV), want_counts=True, **kw)
+        _check(z, k, scoring, torch.zeros(e), kw, torch.float32, got)
+        one = torch.cat([_ops().route_topk(z[p:p + 1].to(DEV), k, scoring, torch.zeros(e, device=DEV), **kw)[1] for p in range(k)])
+        assert torch.equal(one, got[1])                    # (alone in its wave)
+
+
 @pytest.mark.parametrize('e', [4, 8, 16, 64, 200, 1024])
 def test_biases_of_any_size(e):
     """What the choice goes by spans anything from a float32 step of a large offset to the ends of the type: the choice is still
