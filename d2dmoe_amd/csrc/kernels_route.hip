@@ -949,8 +949,18 @@ hipError_t forward_t(const d2dmoe_route_shape& sh, const void* logits, const flo
     const T* z = (const T*)logits;
     T* r = (T*)routing;
     if (sh.n_experts > 512) return forward_l<T, 16, 64>(sh, z, r, A, s);
-    if (sh.n_experts <= 16 && sh.k <= 4)   // (fewer experts per lane: 2^20 rows of 8 are 33 MB and 31 us at eight per lane)
-      return sh.n_experts <= 8 ? forward_l<T, 2, 4>(sh, z, r, A, s) : forward_l<T, 4, 4>(sh, z, r, A, s);
+    // fewer experts per lane where the places ask for so many lanes that four each are enough, or two (at eight per lane 2^20
+    // rows of 8, two each, take 31 us instead of 20, and 135823 x 48 bf16 in groups with a bias, 12 each, 59 instead of 41)
+    const int lanes = team_lanes(1, 8, sh.k);
+    if (sh.n_experts <= 4 * lanes) {
+      switch (lanes) {
+        case 4: return sh.n_experts <= 8 ? forward_l<T, 2, 4>(sh, z, r, A, s) : forward_l<T, 4, 4>(sh, z, r, A, s);
+        case 8: return forward_l<T, 4, 8>(sh, z, r, A, s);
+        case 16: return forward_l<T, 4, 16>(sh, z, r, A, s);
+        case 32: return forward_l<T, 4, 32>(sh, z, r, A, s);
+        default: return forward_l<T, 4, 64>(sh, z, r, A, s);
+      }
+    }
     switch (team_lanes(sh.n_experts, 8, sh.k)) {
       case 4: return forward_l<T, 8, 4>(sh, z, r, A, s);
       case 8: return forward_l<T, 8, 8>(sh, z, r, A, s);

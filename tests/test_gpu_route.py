@@ -116,6 +116,22 @@ def test_groups_and_bias(e, groups, kept, k, t):
                 _check(z, k, scoring, bias, kw, t, got)
 
 
+@pytest.mark.parametrize('t', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('e,groups,k', [(5, 1, 5), (16, 2, 8), (18, 3, 5), (32, 4, 8), (33, 3, 9), (20, 2, 16), (48, 8, 12), (60, 5, 9), (64, 8, 16), (65, 5, 12),
+                                        (64, 4, 32), (100, 10, 30), (128, 4, 32), (130, 2, 20), (66, 3, 33), (200, 8, 50), (256, 8, 64), (257, 1, 40)])
+def test_many_places(e, groups, k, t):
+    """Nearly as many places as the experts, and the lanes of their teams, leave room for."""
+    for scoring in ('softmax', 'sigmoid'):
+        for biased in (False, True):
+            for kept in sorted({groups, -(-k * groups // e)}):
+                print('places', e, groups, kept, k, t, scoring, biased, flush=True)
+                z = _logits(21, e, t, seed=e + k, masks=True)
+                bias = torch.randn(e, generator=torch.Generator().manual_seed(k)) * 0.1 if biased else None
+                kw = dict(n_groups=groups, kept_groups=kept, group_score='top2' if biased else 'max', renormalise=True, scale=1.5)
+                got = _ops().route_topk(z.to(DEV), k, scoring, None if bias is None else bias.to(DEV), want_counts=True, **kw)
+                _check(z, k, scoring, bias, kw, t, got)
+
+
 def test_bias_that_is_not_a_number_routes_nothing():
     z = _logits(9, 32, torch.float32, seed=1)
     bias = torch.zeros(32)
