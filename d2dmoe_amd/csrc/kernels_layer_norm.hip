@@ -21,10 +21,10 @@ constexpr int NT = 256;   // threads per workgroup
 
 // ---------------------------------------------------------------------------------------------------------------------
 // A row in registers.  TPR threads per row: a part of a wave (8, 16 or 32 lanes: narrow rows, several per wave), one wave, or a
-// whole workgroup of 256 or 1024 (the only ones with a barrier), CH vectors of 16 bytes each.  All but the last of the CH are whole; in the last one a thread may lie behind the row's end (it reads
-// the row's first vector and drops it) or across it (it reads the row's last whole vector, of which it counts the elements
-// nobody else has; the others are computed twice and stored twice, with the same bits).  Rows may begin at any element: the
-// loads and stores make no claim on alignment.
+// whole workgroup of 256, 512 or 1024 (the only ones with a barrier), CH vectors of 16 bytes each.  All but the last of the CH
+// are whole; in the last one a thread may lie behind the row's end (it reads the row's first vector and drops it) or across it
+// (it reads the row's last whole vector, of which it counts the elements nobody else has; the others are computed twice and
+// stored twice, with the same bits).  Rows may begin at any element: the loads and stores make no claim on alignment.
 //
 // Bound by HBM: a row is read once and written once.  bf16 with residual, 50432 x 768: 60 us, 5.1 TB/s (this card copies at
 // 4.9 to 5.5 TB/s); 32768 x 4096 with statistics: 195 us, 5.5 TB/s; 65536 x 64: 6.7 us, 5.0 TB/s.  With one row per workgroup
@@ -218,7 +218,7 @@ struct NormBackward {
 template <typename T, typename P, int TPR, int CH>
 __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void layer_norm_grad_kernel(const NormBackward A) {
   constexpr int V = kVec<T>, RPW = kRowsPerWave<TPR>, Q = 2 * CH * V / 4;
-  constexpr bool AHEAD = TPR < 1024;      // (1024 threads leave 128 registers each: the row is requested when it is due)
+  constexpr bool AHEAD = TPR < 1024 && CH < 4;   // (registers: the row is requested when it is due)
   __shared__ float buf[2][2][kWaves<TPR>];
   __shared__ float4 sums[TPR <= 64 ? 2 : 1][TPR <= 64 ? Q : 1][64];
   int turn = 0;
@@ -498,8 +498,10 @@ inline int slab_count(int64_t N) { return (int)(N < 64 ? 1 : (cdiv64(N, 64) < 25
 
 // Threads per row and vectors per thread for a width, or TPR = 0 where the row does not fit: as few lanes as one vector each is
 // enough for (65536 rows of 64 bf16: 23 us with a wave each), then a wave per row as long as `most` vectors per thread are
-// enough, then a workgroup of 256, of 1024.  Forward four; backward three, whose sums and the row ahead make 228 of the 256
-// registers that two workgroups per CU leave each thread (1024 threads have 128, room for one, two with spills).
+// enough, then a workgroup of 256, of 1024.  Forward four; backward three, whose sums and the row ahead make 240 of the 256
+// registers that two waves per SIMD leave each thread.  There 1024 threads have 128, room for one vector (8192 x 8192 bf16:
+// 110 us), and wider rows take 512 threads: 8192 x 12288 bf16 160 us (5.0 TB/s), with 1024 threads of two vectors, which spilled,
+// 471; four vectors spill up to 24 registers and wait for their row (8192 x 16384: 250 us, 4.3 TB/s).
 struct RowPlan { int tpr, ch; };
 template <typename T> RowPlan row_plan(int D, bool forward) {
   constexpr int V = kVec<T>;
@@ -508,7 +510,8 @@ template <typename T> RowPlan row_plan(int D, bool forward) {
   if (vectors <= 32) return {vectors <= 8 ? 8 : vectors <= 16 ? 16 : 32, 1};
   if (vectors <= 64 * most) return {64, (vectors + 63) / 64};
   if (vectors <= 256 * most) return {256, (vectors + 255) / 256};
-  if (vectors <= 1024 * (forward ? 4 : 2)) return {1024, (vectors + 1023) / 1024};
+  if (vectors <= 1024 * (forward ? 4 : 1)) return {1024, (vectors + 1023) / 1024};
+  if (!forward && vectors <= 512 * 4) return {512, (vectors + 511) / 512};
   return {0, 0};
 }
 
@@ -519,7 +522,7 @@ inline unsigned row_grid(int64_t N, int rows, int per_cu) {
   return (unsigned)(need < most ? need : most);
 }
 // The gradient's: every workgroup leaves 2 D sums behind, so each takes four rows per wave or row team at least.
-inline int grad_parts(const d2dmoe_norm_shape& sh, int tpr) { return (int)row_grid(sh.n_rows, 4 * (tpr < NT ? NT / tpr : 1), tpr == 1024 ? 1 : 2); }
+inline int grad_parts(const d2dmoe_norm_shape& sh, int tpr) { return (int)row_grid(sh.n_rows, 4 * (tpr < NT ? NT / tpr : 1), tpr >= 512 ? 1 : 2); }
 
 template <typename T, typename P, int TPR, int CH>
 hipError_t forward_rows(const NormForward& A, hipStream_t s) {
@@ -547,9 +550,8 @@ hipError_t backward_rows(const NormBackward& A, unsigned grid, hipStream_t s) {
     case 256 * 8 + 1: e = CALL(256, 1); break;      \
     case 256 * 8 + 2: e = CALL(256, 2); break;      \
     case 256 * 8 + 3: e = CALL(256, 3); break;      \
-    case 1024 * 8 + 1: e = CALL(1024, 1); break;    \
     EXTRA                                           \
-    default: e = CALL(1024, 2); break;              \
+    default: e = CALL(1024, 1); break;              \
   }
 
 template <typename T, typename P>
@@ -561,7 +563,8 @@ hipError_t forward_t(const d2dmoe_norm_shape& sh, const void* x, const void* res
     const NormForward A{x, residual, weight, bias, sum, out, mean, rstd, sh.n_rows, sh.width, sh.eps};
 #define D2DMOE_ROWS(TPR, CH) forward_rows<T, P, TPR, CH>(A, s)
     D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, case 64 * 8 + 4: e = D2DMOE_ROWS(64, 4); break;
-                        case 256 * 8 + 4: e = D2DMOE_ROWS(256, 4); break; case 1024 * 8 + 3: e = D2DMOE_ROWS(1024, 3); break;
+                        case 256 * 8 + 4: e = D2DMOE_ROWS(256, 4); break;
+                        case 1024 * 8 + 2: e = D2DMOE_ROWS(1024, 2); break; case 1024 * 8 + 3: e = D2DMOE_ROWS(1024, 3); break;
                         case 1024 * 8 + 4: e = D2DMOE_ROWS(1024, 4); break;)
 #undef D2DMOE_ROWS
     return e;
@@ -585,7 +588,8 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
     parts = grad_parts(sh, plan.tpr);
     const NormBackward A{g, gs, h, weight, mean, rstd, grad, columns ? (float*)workspace : nullptr, N, D};
 #define D2DMOE_ROWS(TPR, CH) backward_rows<T, P, TPR, CH>(A, (unsigned)parts, s)
-    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, )
+    D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, case 512 * 8 + 3: e = D2DMOE_ROWS(512, 3); break;
+                        case 512 * 8 + 4: e = D2DMOE_ROWS(512, 4); break;)
 #undef D2DMOE_ROWS
   } else if (N > 0) {
     if (grad != nullptr) {

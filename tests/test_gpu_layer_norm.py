@@ -118,6 +118,13 @@ def test_forward_and_backward(n, d, t, p):
         assert all(torch.equal(a, c) for a, c in zip(got, again))
 
 
+@pytest.mark.parametrize('t,p', TYPES)
+@pytest.mark.parametrize('n,d', [(270, 12288), (259, 10001), (258, 16381), (3, 8193), (262, 4100), (260, 7383)])
+def test_wide_rows_in_turn(n, d, t, p):
+    """More wide rows than workgroups: each takes several, one after the other."""
+    test_forward_and_backward(n, d, t, p)
+
+
 @pytest.mark.parametrize('d', [768, 77])
 def test_optional_operands(d):
     """Each of weight, bias and the outputs may be missing; what is there does not change."""
