@@ -54,12 +54,13 @@ __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 // other score of a pair shares; sigmoid: 4.2 u) and its sum with a bias by u |c| more.  Where two choices whose order matters
 // lie within 2^-19 + 2^-22 |c| of each other (sums of two scores: twice that) -- places next to one another in the list, the
 // last place and the first one left out, a group that stays and one that goes -- the wave repeats its choice on float64
-// scores; a row or two in a thousand do.  Their waves finish last: 16384 x 256 takes 16.6 us with a bias, 12 us with one that
-// leaves nothing in doubt, 30 us with one (all zeros, 16-bit logits) that leaves every wave in doubt.
+// scores; a row or two in a thousand do.  Their waves finish last: 16384 x 256 takes 16.8 us with a bias, of which 4.5 us are that
+// tail, and 30 us with one (all zeros, 16-bit logits) that leaves every wave in doubt.
 //
 // Bound by vector instructions, not by memory: 388 per wave of four tokens at 128 experts and 8 places in bf16, 776 per wave
 // of two at 256 in float32 with groups and a bias.  50432 x 128 bf16: 11 us (29 MB: 5.6 us at this card's copy rate);
-// 16384 x 256 float32 in groups: 20 us (35 MB: 6.7 us), 131072 x 256: 85 us.  Before: one wave per token with float64 throughout, 396 and 206 us.
+// 16384 x 256 float32 in groups: 20 us (35 MB: 6.7 us), 131072 x 256: 86 us.  Before: one wave per token with float64
+// throughout, 396 us for the first and 206 us for the second.
 // =====================================================================================================
 constexpr int WAVES = 4;   // per workgroup
 
@@ -468,6 +469,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
     using K = Keys<T, V, !direct ? FIXED : (sizeof(T) == 4 ? WIDE : HALF)>;
     K keys;
     float near_by = 0.f;                                      // FIXED: the doubt in steps
+    bool windowed = false;
     if constexpr (direct) {
 #pragma unroll
       for (int j = 0; j < V; ++j) keys.set(j, by[j], e0 + j);
@@ -480,7 +482,11 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       }
       most = team_max<L>(most);
       least = -team_max<L>(-least);
-      const float range = most - least;                       // (infinite: a scale of 0, and nothing told apart)
+      // Further apart than scores are: masks (the type's lowest value, -1e9) in the bias.  Only the uppermost part is told apart
+      // then, and a place that falls below it or next to its end is in doubt (16384 x 256 with a tenth masked so: 31 us without, 17 us).
+      windowed = !(most - least <= 64.f) && most > -INFINITY;
+      least = windowed ? most - 4.f : least;
+      const float range = most - least;
       const float scale = fminf((kTop - 2.f * kMargin) * __builtin_amdgcn_rcpf(fmaxf(range, 0x1p-80f)), 0x1p100f);
       const float offset = kMargin - least * scale;
       near_by = (0x1p-19f + 0x1p-22f * fmaxf(fabsf(most), fabsf(least))) * scale + 2.f;
@@ -520,6 +526,7 @@ __global__ __launch_bounds__(WAVES * 64) void route_team_kernel(const T* __restr
       const uint32_t after = (uint32_t)__shfl_down((int)mine_lo, 1, kWave);   // (by all lanes: a lane that is switched off gives 0)
       const uint32_t next = tl == A.K - 1 ? lo : after;
       if (tl < A.K && next >= kNone && (float)((mine_lo >> 10) - (next >> 10)) <= near_by) doubt = true;
+      if (tl < A.K && windowed && (float)(mine_lo >> 10) <= kMargin + near_by) doubt = true;
       if (__ballot(doubt) != 0ull) at = choose_exactly<V, L, groups>(z, bad, A, (double*)lds);
       // the chosen logits come out of the lanes that hold them through LDS
       float* zs = (float*)lds + team * (L * V);

@@ -159,6 +159,26 @@ def test_neighbours_that_float32_scores_do_not_tell_apart(scoring):
     _check(zb[:400], 8, scoring, torch.zeros(64), {}, torch.bfloat16, (got[0][:400], got[1][:400], got[2][:400], None))
 
 
+@pytest.mark.parametrize('e,k', [(8, 3), (16, 12), (64, 8), (200, 8), (256, 24), (1024, 8)])
+def test_masks_in_the_bias(e, k):
+    """Low values that switch experts off, also so many that some of those have to be chosen, and choices a little above and below
+    a distance of four from the best."""
+    g = torch.Generator().manual_seed(e)
+    z = _logits(60 if e <= 256 else 20, e, torch.float32, seed=e)
+    z[1::3] = z[1::3, :1]                                      # rows of equal logits
+    some = torch.rand(e, generator=g)
+    for off in (torch.finfo(torch.float32).min, -1e9, -1e4, -65.0, -4.0, -3.0):
+        for share in (0.1, 0.9, 1.0):
+            bias = torch.where(some < share, off, 0.0)
+            bias[e // 2] = -62.0 if off < -65 else 0.5
+            bias[e // 3] = max(off, -1e4) + 61.0
+            for scoring in ('softmax', 'sigmoid'):
+                for kw in ({}, dict(n_groups=4, kept_groups=3, group_score='top2')):
+                    print('mask', e, k, off, share, scoring, kw, flush=True)
+                    got = _ops().route_topk(z.to(DEV), k, scoring, bias.to(DEV), want_counts=True, **kw)
+                    _check(z, k, scoring, bias, kw, torch.float32, got)
+
+
 @pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
 @pytest.mark.parametrize('e,k', [(2, 1), (4, 2), (8, 4), (16, 4), (24, 4), (64, 8), (128, 8), (256, 8), (256, 32), (512, 8), (1000, 20), (1024, 64)])
 def test_one_pair_that_float32_scores_do_not_tell_apart(e, k, scoring):
