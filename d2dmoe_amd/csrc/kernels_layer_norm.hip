@@ -206,6 +206,7 @@ struct NormBackward {
   const float *mean, *rstd;
   void* grad;
   float* partial;   // [workgroup][2][D]: column sums of the workgroup's rows, or NULL
+  void *gw, *gb;    // a single workgroup's column sums are the result: either may be NULL
   int64_t N;
   int D;
 };
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
       }
     }
   }
-  if (A.partial == nullptr) return;
+  if (A.partial == nullptr && A.gw == nullptr && A.gb == nullptr) return;
   float* flat = &cs[0][0][0];
   if constexpr (TPR <= 64) {
     // the wave's rows first, where it has several
@@ -340,6 +341,19 @@ __global__ __launch_bounds__(TPR < NT ? NT : TPR, TPR == 1024 ? 1 : 2) void laye
     __syncthreads();
     if (wave != 0 || lane >= TPR) return;
     add(0);
+  }
+  if (A.partial == nullptr) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      P* out = (P*)(k == 0 ? A.gw : A.gb);
+      if (out == nullptr) continue;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c < CH - 1 || j >= skip) Elem<P>::store(out + at[c] + j, cs[k][c][j]);
+    }
+    return;
   }
   float* out = A.partial + (int64_t)blockIdx.x * 2 * D;
 #pragma unroll
@@ -586,7 +600,9 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
   const RowPlan plan = row_plan<T>(D, false);
   if (N > 0 && plan.tpr != 0) {
     parts = grad_parts(sh, plan.tpr);
-    const NormBackward A{g, gs, h, weight, mean, rstd, grad, columns ? (float*)workspace : nullptr, N, D};
+    const bool one = parts == 1;       // (16 rows of 768: one launch of two)
+    const NormBackward A{g, gs, h, weight, mean, rstd, grad, columns && !one ? (float*)workspace : nullptr, one ? gw : nullptr,
+                         one ? gb : nullptr, N, D};
 #define D2DMOE_ROWS(TPR, CH) backward_rows<T, P, TPR, CH>(A, (unsigned)parts, s)
     D2DMOE_ROW_DISPATCH(plan, D2DMOE_ROWS, case 512 * 8 + 3: e = D2DMOE_ROWS(512, 3); break;
                         case 512 * 8 + 4: e = D2DMOE_ROWS(512, 4); break;)
@@ -605,7 +621,7 @@ hipError_t backward_t(const d2dmoe_norm_shape& sh, const void* g, const void* gs
       e = hipGetLastError();
     }
   }
-  if (e != hipSuccess || !columns) return e;
+  if (e != hipSuccess || !columns || (N > 0 && plan.tpr != 0 && parts == 1)) return e;
   hipLaunchKernelGGL((layer_norm_grad_finish_kernel<P>), dim3((unsigned)((2 * D + 31) / 32)), dim3(1024), 0, s,
                      (const float*)workspace, (P*)gw, (P*)gb, parts, D);
   return hipGetLastError();

@@ -6,6 +6,8 @@ scripts/test_moe_implementations.py:78-83)."""
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
+from operator import index as whole
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -429,6 +431,13 @@ def _norm_params(what: str, d: int, dtype: torch.dtype, weight: Optional[torch.T
     return _DTYPES[kind]
 
 
+@lru_cache(maxsize=1024)
+def _norm_shape(n: int, d: int, code: int, pcode: int, eps: float):
+    """A call's shape by reference and the bytes of its backward workspace, which follow from these numbers alone (1.7 us to make)."""
+    sh = ctypes.byref(abi.NormShape(n, d, code, pcode, eps))
+    return sh, abi.load().d2dmoe_layer_norm_workspace_bytes(sh)
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                residual: Optional[torch.Tensor] = None, want_stats: bool = False):
     """Layer norm of the rows of x [N,D], or of h = x + residual (rounded to the storage type), through d2dmoe_layer_norm.
@@ -447,8 +456,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     mean = rstd = None
     if want_stats:
         mean, rstd = torch.empty(2, n, dtype=torch.float32, device=x.device).unbind(0)
-    sh = abi.NormShape(n, d, code, pcode, eps)
-    _launch(index, lib.d2dmoe_layer_norm, 'd2dmoe_layer_norm', ctypes.byref(sh), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
+    sh, _ = _norm_shape(n, d, code, pcode, float(eps))
+    _launch(index, lib.d2dmoe_layer_norm, 'd2dmoe_layer_norm', sh, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias),
             _ptr(total), out.data_ptr(), _ptr(mean), _ptr(rstd))
     return out, total, mean, rstd
 
@@ -484,27 +493,31 @@ def layer_norm_backward(grad_out: torch.Tensor, h: torch.Tensor, weight: Optiona
     gb = torch.empty(d, dtype=ptype, device=dev) if want_bias else None
     if grad is None and gw is None and gb is None:
         return None, None, None
-    sh = abi.NormShape(n, d, code, pcode, 0.0)
-    ws, nbytes = None, 0
-    if gw is not None or gb is not None:
+    sh, nbytes = _norm_shape(n, d, code, pcode, 0.0)
+    ws = None
+    if nbytes > 0 and (gw is not None or gb is not None):
         # (a buffer of this call's own, not the one kept per stream: a captured call keeps its buffer with its graph)
-        nbytes = lib.d2dmoe_layer_norm_workspace_bytes(ctypes.byref(sh))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(index, lib.d2dmoe_layer_norm_backward, 'd2dmoe_layer_norm_backward', ctypes.byref(sh), grad_out.data_ptr(), _ptr(grad_sum),
+    _launch(index, lib.d2dmoe_layer_norm_backward, 'd2dmoe_layer_norm_backward', sh, grad_out.data_ptr(), _ptr(grad_sum),
             h.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(grad), _ptr(gw), _ptr(gb), _ptr(ws), nbytes)
     return grad, gw, gb
 
 
+@lru_cache(maxsize=1024)
+def _route_record(*numbers):
+    return ctypes.byref(abi.RouteShape(*numbers))
+
+
 def _route_shape(what: str, logits: torch.Tensor, k: int, scoring: str, renormalise: bool, scale: float, n_groups: int = 1,
-                 kept_groups: int = 1, group_score: str = 'top2') -> abi.RouteShape:
+                 kept_groups: int = 1, group_score: str = 'top2'):
     code = _dtype_code(logits)
     if logits.dim() != 2:
         raise abi.D2DMoEError(f'{what}: logits have {logits.dim()} dimensions, expected [N,E]')
     if scoring not in abi.SCORING or group_score not in abi.GROUP_SCORE:
         raise abi.D2DMoEError(f'{what}: scoring is one of {sorted(abi.SCORING)}, group_score one of {sorted(abi.GROUP_SCORE)}')
     n, e = logits.shape
-    return abi.RouteShape(n, e, k, code, abi.SCORING[scoring], n_groups, kept_groups, abi.GROUP_SCORE[group_score],
-                          1 if renormalise else 0, scale)
+    return _route_record(n, e, whole(k), code, abi.SCORING[scoring], whole(n_groups), whole(kept_groups), abi.GROUP_SCORE[group_score],
+                         1 if renormalise else 0, float(scale))
 
 
 def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bias: Optional[torch.Tensor] = None,
@@ -526,7 +539,7 @@ def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bi
     indices = torch.empty(n, k, dtype=torch.int32, device=dev)
     weights = torch.empty(n, k, dtype=torch.float32, device=dev)
     counts = torch.empty(e, dtype=torch.int32, device=dev) if want_counts else None
-    _launch(index, lib.d2dmoe_route_topk, 'd2dmoe_route_topk', ctypes.byref(sh), logits.data_ptr(), _ptr(choice_bias),
+    _launch(index, lib.d2dmoe_route_topk, 'd2dmoe_route_topk', sh, logits.data_ptr(), _ptr(choice_bias),
             routing.data_ptr(), indices.data_ptr(), weights.data_ptr(), _ptr(counts))
     return routing, indices, weights, counts
 
@@ -550,6 +563,6 @@ def route_topk_backward(logits: torch.Tensor, indices: torch.Tensor, scoring: st
     index = _gpu_index(logits, indices, grad_routing, grad_weights)
     lib = abi.load()
     grad = torch.empty_like(logits)
-    _launch(index, lib.d2dmoe_route_topk_backward, 'd2dmoe_route_topk_backward', ctypes.byref(sh), logits.data_ptr(), indices.data_ptr(),
+    _launch(index, lib.d2dmoe_route_topk_backward, 'd2dmoe_route_topk_backward', sh, logits.data_ptr(), indices.data_ptr(),
             _ptr(grad_routing), _ptr(grad_weights), grad.data_ptr())
     return grad
