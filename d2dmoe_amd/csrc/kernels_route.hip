@@ -258,11 +258,19 @@ __device__ inline float add_best(float a, float b) { return max1(a + b, -0x1.fff
 __device__ inline double add_best(double a, double b) { return a + b; }
 template <typename C>
 __device__ __forceinline__ C group_score(const RouteArgs& A, C a, C b) { return (A.top2 && b > -(C)INFINITY) ? add_best(a, b) : a; }
+// Two large choices of opposite signs: each is off by u times its own size, which their small sum does not show, so the sum's place
+// is in doubt wherever it lies.  Below that line two such scores differ by up to 50 u from the scores they add (see above), 8 u
+// and 5 u of the sum's size from its two roundings and the choices': within the 64 u and 8 u of a score that rank_groups asks for.
+__device__ __forceinline__ bool cancels(const RouteArgs& A, float a, float b) {
+  return A.top2 && b > -INFINITY && fabsf(a) + fabsf(b) > fmaf(1.5f, fabsf(a + b), 4.f);
+}
+__device__ __forceinline__ bool cancels(const RouteArgs&, double, double) { return false; }   // (the scores that decide)
 
-// The scores of the T G groups from the choices in tile[] (T rows of E).
+// The scores of the T G groups from the choices in tile[] (T rows of E); returns whether one of them cancels.
 template <typename C, int T>
-__device__ __forceinline__ void score_groups(const C* tile, C* score, const RouteArgs& A) {
+__device__ __forceinline__ bool score_groups(const C* tile, C* score, const RouteArgs& A) {
   const C low = -(C)INFINITY;
+  bool lost = false;
   for (int p = threadIdx.x & 63; p < T * A.G; p += 64) {
     const C* q = tile + p * A.size;       // token-major, groups in order: p counts both
     C a = low, b = low;
@@ -272,7 +280,9 @@ __device__ __forceinline__ void score_groups(const C* tile, C* score, const Rout
       a = larger(a, v);
     }
     score[p] = group_score(A, a, b);
+    lost = lost || cancels(A, a, b);
   }
+  return lost;
 }
 
 // Drops the groups that do not stay from by[] (-inf); returns whether a group's place was in doubt (NEAR).  tile: T E values,
@@ -283,6 +293,7 @@ __device__ __forceinline__ bool keep_groups(C (&by)[V], const RouteArgs& A, C ne
   const int lane = threadIdx.x & 63, tl = lane & (L - 1), team = lane / L;
   const int size = A.size, G = A.G, e0 = tl * V;
   const C low = -(C)INFINITY;
+  bool lost = false;
   wave_sync();
   if (size % V == 0) {
     // whole lanes per group: the two largest of ever longer runs of lanes, up to the group's end, in its first lane
@@ -300,17 +311,21 @@ __device__ __forceinline__ bool keep_groups(C (&by)[V], const RouteArgs& A, C ne
         a = larger(a, oa);
       }
     }
-    if (pos == 0 && e0 < A.E) score[team * G + of] = group_score(A, a, b);
+    if (pos == 0 && e0 < A.E) {
+      score[team * G + of] = group_score(A, a, b);
+      if constexpr (NEAR) lost = cancels(A, a, b);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (e0 + j < A.E) tile[team * A.E + e0 + j] = by[j];
     wave_sync();
-    score_groups<C, T>(tile, score, A);
+    lost = score_groups<C, T>(tile, score, A);
   }
   wave_sync();
   uint8_t* stays = (uint8_t*)tile;
-  const bool doubt = rank_groups<C, T, NEAR>(score, stays, A, near_abs, near_rel);
+  bool doubt = rank_groups<C, T, NEAR>(score, stays, A, near_abs, near_rel);
+  if constexpr (NEAR) doubt = doubt || __ballot(lost) != 0ull;
   wave_sync();
   int g = small_div(e0, A.inv_size);
   if (size % V == 0) {

@@ -222,6 +222,29 @@ def test_biases_of_any_size(e):
                 _check(z, k, scoring, bias, kw, torch.float32, got)
 
 
+@pytest.mark.parametrize('e,groups', [(8, 2), (24, 4), (64, 4), (256, 8), (1024, 16)])
+def test_large_biases_that_cancel_in_a_group(e, groups):
+    """In every group one expert that a bias of +B forces and one that -B masks, as its two best: the sum is a few units, each
+    addend's float32 rounding B 2^-24, so the order of two sums may only come from the float64 ones."""
+    g = torch.Generator().manual_seed(e)
+    size = e // groups
+    n = max(300, 24000 // e)
+    for large in (1e2, 1e3, 1e4, 1e5, 1e7):
+        for spread in (1.5, 0.02):
+            z = torch.randn(n, e, generator=g) * spread
+            bias = torch.full((e,), -2.0 * large)
+            for i in range(groups):
+                at = torch.randperm(size, generator=g)[:2] + i * size
+                own = large * (1 + 0.25 * (i % 2))
+                bias[at[0]], bias[at[1]] = own, -own
+            for scoring in ('softmax', 'sigmoid'):
+                for kept, k in ((1, 1), (groups // 2, min(2, groups // 2))):
+                    kw = dict(n_groups=groups, kept_groups=kept, group_score='top2')
+                    print('cancel', e, groups, large, spread, scoring, kept, k, flush=True)
+                    got = _ops().route_topk(z.to(DEV), k, scoring, bias.to(DEV), want_counts=True, **kw)
+                    _check(z, k, scoring, bias, kw, torch.float32, got)
+
+
 def test_scores_that_underflow_still_share_their_weight():
     """Chosen scores of 1e-60 and less: renormalised weights go by their ratio."""
     z = torch.tensor([[-140.0, -139.0, -150.0, -400.0], [-3e38, -3e38, -3e38, -3e38]])
