@@ -391,7 +391,7 @@ def _gpu_index(*tensors: Optional[torch.Tensor]) -> int:
         if t is None:
             continue
         i = t.get_device()       # -1 off the GPU
-        if i != index:
+        if i != index or i < 0:  # (i < 0: also ahead of the first tensor on a GPU)
             if i < 0:
                 raise abi.D2DMoEError('the HIP path needs tensors on a ROCm device; there is no CPU fallback')
             if index >= 0:

@@ -270,6 +270,31 @@ def test_a_call_runs_on_its_tensors_device(monkeypatch):
     assert seen == [(7, 1000)]
 
 
+class _Standin:
+    """A tensor as far as the device check goes; -1: on the CPU."""
+
+    def __init__(self, index, contiguous=True):
+        self.index, self.contiguous = index, contiguous
+
+    def get_device(self):
+        return self.index
+
+    def is_contiguous(self):
+        return self.contiguous
+
+
+def test_device_check_in_any_order():
+    """A tensor on the CPU is refused wherever it stands among tensors on a GPU: its address would reach the kernel."""
+    from d2dmoe_amd import D2DMoEError, ops
+    for where in ((-1, 0), (0, -1), (-1, -1), (None, -1, 0), (-1, None, 0, 0), (0, None, -1), (0, 1), (1, 0), (None, 2, 2, 3), (None,), ()):
+        with pytest.raises(D2DMoEError):
+            ops._gpu_index(*(None if i is None else _Standin(i) for i in where))
+    for where, index in (((0,), 0), ((None, 3, None, 3), 3), ((1, 1, 1), 1)):
+        assert ops._gpu_index(*(None if i is None else _Standin(i) for i in where)) == index
+    with pytest.raises(D2DMoEError):
+        ops._gpu_index(_Standin(0), _Standin(0, contiguous=False))
+
+
 def test_tensor_level_refusals():
     from d2dmoe_amd import D2DMoEError, functional, ops
     x = torch.randn(4, 8)
