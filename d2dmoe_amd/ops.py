@@ -431,9 +431,17 @@ def _norm_params(what: str, d: int, dtype: torch.dtype, weight: Optional[torch.T
     return _DTYPES[kind]
 
 
+def _fits_32_bits(*numbers: int) -> None:
+    """ctypes cuts a number to its field without a word, so what the library checks would be another number."""
+    for v in numbers:
+        if not -(1 << 31) <= v < 1 << 31:
+            raise abi.D2DMoEError(f'a size of {v} does not fit the 32 bits that the library takes it in')
+
+
 @lru_cache(maxsize=1024)
 def _norm_shape(n: int, d: int, code: int, pcode: int, eps: float):
     """A call's shape by reference and the bytes of its backward workspace, which follow from these numbers alone (1.7 us to make)."""
+    _fits_32_bits(d)
     sh = ctypes.byref(abi.NormShape(n, d, code, pcode, eps))
     return sh, abi.load().d2dmoe_layer_norm_workspace_bytes(sh)
 
@@ -505,6 +513,7 @@ def layer_norm_backward(grad_out: torch.Tensor, h: torch.Tensor, weight: Optiona
 
 @lru_cache(maxsize=1024)
 def _route_record(*numbers):
+    _fits_32_bits(*numbers[1:-1])
     return ctypes.byref(abi.RouteShape(*numbers))
 
 

@@ -270,6 +270,21 @@ def test_a_call_runs_on_its_tensors_device(monkeypatch):
     assert seen == [(7, 1000)]
 
 
+def test_numbers_beyond_32_bits_are_refused_not_cut():
+    """The C records hold 32-bit fields, and ctypes drops what does not fit: 2^32 + 1 groups would run as one."""
+    from d2dmoe_amd import D2DMoEError, ops
+    x = torch.randn(4, 8)
+    for far in (1 << 32, (1 << 32) + 1, (1 << 31), -(1 << 32) + 1):
+        for args in (dict(n_groups=far), dict(kept_groups=far), dict(k=far)):
+            with pytest.raises(D2DMoEError, match='32 bits'):
+                ops._route_shape('route_topk', x, **{**dict(k=2, scoring='softmax', renormalise=True, scale=1.0), **args})
+    with pytest.raises(D2DMoEError, match='32 bits'):
+        ops._route_record(4, (1 << 32) + 8, 2, 0, 0, 1, 1, 0, 1, 1.0)
+    with pytest.raises(D2DMoEError, match='32 bits'):
+        ops._norm_shape(1, (1 << 32) + 8, 1, 1, 1e-5)
+    assert ops._norm_shape(1 << 40, 8, 1, 1, 1e-5)[0]._obj.n_rows == 1 << 40      # (rows and tokens are 64-bit)
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 
