@@ -1,7 +1,7 @@
 """The operators of this package that have a backward pass, as differentiable functions on ROCm tensors: layer norm (with
 the residual added ahead of it) and routing by scores.  Forward and backward are the HIP kernels behind ``ops``; what is
 saved for the backward pass is the normalised tensor with its row statistics, or the logits with the chosen indices.
-Where no gradient is asked for, nothing is saved.  Double backward is not supported.
+Where no gradient is asked for, nothing is saved.  Double backward is not supported; forward-mode derivatives are refused.
 
 Capturing a training step into a HIP graph: PyTorch ties a parameter's gradient accumulator to the stream on which the first
 graph that reaches it was built, so capture before an eager graph of the same parameters is alive (or after it has been
@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -63,6 +64,11 @@ class _RouteTopk(torch.autograd.Function):
 
 
 def _wanted(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a reverse-mode gradient is asked for.  Forward mode shows in no requires_grad: a tensor with a tangent would come
+    out of the kernels without one, so it is refused here (looked for inside a dual level only: 0.3 us a tensor)."""
+    if getattr(forward_ad, '_current_level', 0) >= 0 and \
+            any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError('layer_norm and route_topk have no forward-mode derivative')
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

@@ -285,6 +285,28 @@ def test_numbers_beyond_32_bits_are_refused_not_cut():
     assert ops._norm_shape(1 << 40, 8, 1, 1, 1e-5)[0]._obj.n_rows == 1 << 40      # (rows and tokens are 64-bit)
 
 
+def test_forward_mode_derivatives_are_refused_not_lost(monkeypatch):
+    """A dual tensor that asks for no reverse-mode gradient must not come out without its tangent.  The kernel calls are replaced:
+    what is tested is what stands in front of them."""
+    from d2dmoe_amd import functional, ops
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(ops, 'layer_norm', lambda x, w, b, eps, r, want_stats=False: (x * 1.0, None if r is None else x + r, None, None))
+    monkeypatch.setattr(ops, 'route_topk', lambda z, k, *args: (z * 1.0, torch.zeros(z.size(0), k, dtype=torch.int32),
+                                                               torch.ones(z.size(0), k), None))
+    x, w = torch.randn(4, 8), torch.ones(8)
+    with forward_ad.dual_level():
+        dual, dual_w = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, w)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: functional.layer_norm(dual, w), lambda: functional.layer_norm(x, w, residual=dual),
+                             lambda: functional.layer_norm(x, dual_w), lambda: functional.layer_norm(x, w, dual_w),
+                             lambda: functional.route_topk(dual, 2)):
+                    with pytest.raises(NotImplementedError):
+                        call()
+        # tensors without a tangent pass as ever
+        assert functional.layer_norm(x, w).shape == (4, 8) and functional.route_topk(x, 2)[1].shape == (4, 2)
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 
