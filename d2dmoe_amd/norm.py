@@ -7,6 +7,7 @@ modes round alike at the tensors they store (the residual stream, the norm's out
 latter at most."""
 from __future__ import annotations
 
+import torch
 from torch import nn
 from torch.nn import functional as F
 
@@ -31,10 +32,25 @@ class NormModes:
             raise D2DMoEError("forward_mode 'hip' needs a ROCm device; use 'torch' on the CPU")
         return True
 
+    def _forward_hip(self, x, residual):
+        """The kernels take one element type; what the 'torch' mode takes beside that is brought to it here: a sum of two types
+        has the wider one (autocast: a 16-bit branch on a float32 stream), and autocast runs a norm in float32."""
+        weight, bias = self.weight, self.bias
+        if residual is not None and residual.dtype != x.dtype:
+            wide = torch.promote_types(x.dtype, residual.dtype)
+            x, residual = x.to(wide), residual.to(wide)
+        if torch.is_autocast_enabled('cuda'):
+            weight, bias = (None if p is None else p.float() for p in (weight, bias))
+            if x.dtype != torch.float32:
+                h = x if residual is None else x + residual
+                out = functional.layer_norm(h.float(), weight, bias, self.norm_eps())
+                return out if residual is None else (out, h)
+        return functional.layer_norm(x, weight, bias, self.norm_eps(), residual)
+
     def forward(self, x, residual=None):
         """norm(x), or (norm(x + residual), x + residual)."""
         if self._hip(x):
-            return functional.layer_norm(x, self.weight, self.bias, self.norm_eps(), residual)
+            return self._forward_hip(x, residual)
         h = x if residual is None else x + residual
         out = F.layer_norm(h, (h.size(-1),), self.weight, self.bias, self.norm_eps())
         return out if residual is None else (out, h)

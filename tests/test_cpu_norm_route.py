@@ -1,5 +1,6 @@
 """Layer norm and routing by scores without a GPU: the oracle against independent statements, the PyTorch compositions that
 run off the GPU, the modules' modes, and every refusal (none of which may reach a device)."""
+import contextlib
 import ctypes
 import math
 
@@ -305,6 +306,60 @@ def test_forward_mode_derivatives_are_refused_not_lost(monkeypatch):
                         call()
         # tensors without a tangent pass as ever
         assert functional.layer_norm(x, w).shape == (4, 8) and functional.route_topk(x, 2)[1].shape == (4, 2)
+
+
+def _norm_calls(monkeypatch):
+    """The 'hip' mode off the GPU: the kernel call replaced by its formula, with the refusal of two element types that it has."""
+    from d2dmoe_amd import D2DMoEError, norm, ops
+    seen = []
+
+    def layer_norm(x, w=None, b=None, eps=1e-5, residual=None, want_stats=False):
+        if residual is not None and residual.dtype != x.dtype:
+            raise D2DMoEError('two element types')
+        ops._norm_params('layer_norm', x.size(1), x.dtype, w, b)
+        seen.append((x.dtype, None if residual is None else residual.dtype))
+        h = x if residual is None else x + residual
+        out = F.layer_norm(h.float(), (h.size(1),), None if w is None else w.float(), None if b is None else b.float(), eps).to(x.dtype)
+        return out, None if residual is None else h, None, None
+
+    monkeypatch.setattr(ops, 'layer_norm', layer_norm)
+    monkeypatch.setattr(norm.NormModes, '_hip', lambda self, x: self.forward_mode == 'hip')
+    return seen
+
+
+@pytest.mark.parametrize('bias', [True, False])
+def test_hip_norm_takes_the_element_types_of_the_torch_mode(bias, monkeypatch):
+    """Two element types, and autocast: the sum has the wider type, and under autocast the norm is float32."""
+    from d2dmoe_amd import gpt2
+    from d2dmoe_amd.norm import add_norm
+    seen = _norm_calls(monkeypatch)
+    n = gpt2.LayerNorm(16, bias)
+    n.forward_mode = 'hip'
+    x, r = torch.randn(3, 16), torch.randn(3, 16)
+
+    @contextlib.contextmanager
+    def autocast():                                              # (torch's own switches itself off where there is no GPU)
+        with monkeypatch.context() as m:
+            m.setattr(torch, 'is_autocast_enabled', lambda kind: kind == 'cuda')
+            yield
+
+    with torch.no_grad():
+        for tx in (torch.bfloat16, torch.float16, torch.float32):
+            for tr in (torch.bfloat16, torch.float16, torch.float32):
+                wide = torch.promote_types(tx, tr)
+                a, b = x.to(tx), r.to(tr)
+                out, h = add_norm(n, a, b)
+                assert out.dtype == h.dtype == wide and torch.equal(h, a + b) and seen[-1] == (wide, wide)
+                with autocast():
+                    out, h = add_norm(n, a, b)
+                    alone = n(a)
+                # what F.layer_norm gives there on a GPU, and an addition: float32, and the wider type
+                assert out.dtype == alone.dtype == torch.float32 and h.dtype == wide and torch.equal(h, a + b)
+                assert torch.equal(out, F.layer_norm((a + b).float(), (16,), n.weight, n.bias, 1e-5))
+        # 16-bit parameters under autocast, as F.layer_norm takes them
+        n.bfloat16()
+        with autocast():
+            assert n(x).dtype == torch.float32
 
 
 class _Standin:

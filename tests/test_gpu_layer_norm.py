@@ -336,3 +336,66 @@ def test_models_run_on_it():
         assert set(a[1]) == set(c[1])
         for k in a[1]:
             assert (a[1][k] - c[1][k]).norm() <= 1e-3 * a[1][k].norm() + 1e-9, k
+
+
+class _Mix(torch.nn.Module):
+    """In the place of an attention: a projection, which autocast runs in 16 bits."""
+
+    def __init__(self, d, pair):
+        super().__init__()
+        self.project, self.pair = torch.nn.Linear(d, d), pair
+
+    def forward(self, x, *_, **__):
+        out = self.project(x)
+        return (out, None) if self.pair else out
+
+
+@pytest.mark.parametrize('t', [torch.bfloat16, torch.float16])
+def test_models_under_autocast(t):
+    """A training step under autocast: the blocks see a 16-bit branch and a float32 residual stream.  Every norm's input, and with
+    it the stream, has the element type that the PyTorch mode gives it.  The norms' float32 rows differ in their last bits, so a
+    few of the 16-bit roundings behind them flip; were it all of them, a step (twice `half`) each in four norms and as many
+    products, outputs and gradients would be off by 16 `half` of their size.
+
+    A gradient's size is that of the terms it adds up.  The encoder ends in a norm, whose squares add up to D v / (v + eps) in
+    every row: the terms 2 n r of the loss's gradient cancel down to eps of them, the roundings do not.  So the size is
+    taken from the backward pass of a gradient at the output with the same entries under random signs, which keeps every
+    term's size and cancels nothing."""
+    from d2dmoe_amd import gpt2, set_norm_mode, vit
+    torch.manual_seed(0)
+    gpt = gpt2.GPT(gpt2.GPTConfig(block_size=32, vocab_size=64, n_layer=2, n_head=4, n_embd=128)).to(DEV).eval()
+    img = vit.VisionTransformer(image_size=32, num_layers=2, num_heads=4, hidden_dim=128, mlp_dim=256, num_classes=8).to(DEV).eval()
+    for block in gpt.transformer.h:
+        block.attn = _Mix(128, False).to(DEV)
+    for block in img.encoder.layers:
+        block.self_attention = _Mix(128, True).to(DEV)
+    idx = torch.randint(0, 64, (2, 32), device=DEV)
+    tokens = torch.randn(2, 5, 128, device=DEV)
+    for model, data in ((gpt, idx), (img.encoder, tokens)):
+        blocks = list(gpt.transformer.h if model is gpt else img.encoder.layers)
+        results = {}
+        for mode in ('torch', 'hip'):
+            set_norm_mode(model, mode)
+            model.zero_grad()
+            types = []
+            hooks = [b.register_forward_hook(lambda _, i, o: types.append((i[0].dtype, o.dtype))) for b in blocks]
+            with torch.autocast('cuda', t):
+                out = model(data)
+                loss = out.float().square().sum()
+            loss.backward(retain_graph=True)
+            for h in hooks:
+                h.remove()
+            grads = {k: v.grad.clone() for k, v in model.named_parameters() if v.grad is not None}
+            model.zero_grad()
+            signs = torch.randint(0, 2, out.shape, generator=torch.Generator().manual_seed(1)).to(DEV) * 2 - 1
+            out.backward((2 * out.detach().float() * signs).to(out.dtype))
+            sizes = {k: v.grad.norm() for k, v in model.named_parameters() if v.grad is not None}
+            results[mode] = (out.detach().float(), grads, types, sizes)
+        a, c = results['torch'], results['hip']
+        assert a[2] == c[2] and a[2][0][1] == torch.float32
+        bound = 16 * _half(t)
+        assert (a[0] - c[0]).abs().max() <= bound * a[0].abs().max()
+        assert set(a[1]) == set(c[1])
+        for k in a[1]:
+            assert a[1][k].dtype == c[1][k].dtype and torch.isfinite(c[1][k]).all()
+            assert (a[1][k] - c[1][k]).norm() <= bound * torch.maximum(a[1][k].norm(), a[3][k]), k
