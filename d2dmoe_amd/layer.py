@@ -163,7 +163,7 @@ class MoeficationMoE(MoELayer):
     'softmax_topk' and 'sigmoid_topk' take the router's outputs as logits (a router with output_activation='identity') and
     route every token to ``k`` experts with their scores as weights: softmax or sigmoid scores; ``balance_bias`` (float32
     [E] or None) added for the choice only; the experts in ``n_groups`` runs of which ``kept_groups`` stay, scored by
-    ``group_score``; weights renormalised over the chosen when ``renormalise``, times ``route_scale``.  On a ROCm device this
+    ``group_score``; weights renormalised over the chosen when ``renormalise``, times ``route_scale`` (> 0).  On a ROCm device this
     is one HIP kernel with a backward pass of its own, so the router can be trained through the weights."""
 
     def __init__(self, name, hidden_dim, num_experts, bias, expert_dim, activation, experts_class='hip_kernel',
@@ -238,6 +238,8 @@ class MoeficationMoE(MoELayer):
         if mode in self.SCORE_GATES:
             if self.k is None:
                 raise ValueError(f"forward_mode {mode!r} needs k, the number of experts per token")
+            if not 0 < self.route_scale < float('inf'):      # (experts are routed to where the routing tensor is above zero)
+                raise ValueError(f'route_scale is a finite number above zero, got {self.route_scale}')
             logits = self.router(x)
             bias = None if self.balance_bias is None else self.balance_bias.float()
             args = (self.k, self.SCORE_GATES[mode], bias, self.n_groups, self.kept_groups, self.group_score, self.renormalise,

@@ -16,7 +16,8 @@
  *   router_w1  [W, D]      T   first router Linear weight, [out, in] as nn.Linear stores it
  *   router_w2  [E, W]      T   second router Linear weight
  *   norms      [N, E]      T   predicted expert norms = router output
- *   routing    [N, E]      T   routing tensor; the gate writes exactly 0 or 1
+ *   routing    [N, E]      T   routing tensor: a token goes to the experts whose entry is above 0, which is their weight
+ *                              (d2dmoe_select writes exactly 0 or 1, d2dmoe_route_topk the weights of the chosen)
  *   w1         [E, D, Ed]  T   expert up-projections        (gated experts: the gate projection)
  *   b1         [E, Ed]     T   expert first-layer biases, or NULL
  *   w2         [E, Ed, D]  T   expert down-projections
@@ -345,7 +346,7 @@ typedef struct d2dmoe_route_shape {
   int32_t kept_groups;  /* 1 .. n_groups */
   int32_t group_score;  /* D2DMOE_GROUP_* (read with n_groups > 1) */
   int32_t renormalise;  /* 1: the chosen weights of a row add up to scale */
-  float scale;          /* finite */
+  float scale;          /* finite; above 0 where the experts get `routing`, which go by entries above 0 */
 } d2dmoe_route_shape;
 
 /*   choice_bias optional float32 [n_experts]

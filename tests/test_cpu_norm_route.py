@@ -362,6 +362,23 @@ def test_hip_norm_takes_the_element_types_of_the_torch_mode(bias, monkeypatch):
             assert n(x).dtype == torch.float32
 
 
+@pytest.mark.parametrize('mode', ['softmax_topk', 'sigmoid_topk'])
+def test_layer_refuses_a_scale_that_routes_nothing(mode):
+    """The experts count an entry of the routing tensor as routed where it is above zero: with a scale that is not, the containers
+    would disagree ('masked' applies such weights, the others drop every token)."""
+    from d2dmoe_amd import MoeficationMoE, MoeficationRouter
+    moe = MoeficationMoE('m', 16, 8, True, 4, torch.nn.ReLU)
+    moe.router = MoeficationRouter(16, 8, width=16, depth=2, activation='relu', output_activation='identity')
+    moe.forward_mode, moe.k = mode, 3
+    x = torch.randn(2, 5, 16)
+    for scale in (0.0, -1.0, math.nan, -math.inf, math.inf):
+        moe.route_scale = scale
+        with pytest.raises(ValueError, match='route_scale'):
+            moe.gate(x)
+    moe.route_scale = 0.5
+    assert ((moe.gate(x) > 0).sum(-1) == 3).all()
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 
