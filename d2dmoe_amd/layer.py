@@ -20,7 +20,7 @@ from torch import nn
 
 from . import functional, ops
 from .experts import MOE_IMPL_MAP, _HipContainer, _grad_wanted
-from .hip_abi import ACT
+from .hip_abi import ACT, GROUP_SCORE, SCORING, D2DMoEError
 
 
 class _Abs(nn.Module):
@@ -114,11 +114,24 @@ class MoeficationRouter(nn.Module):
         return x
 
 
+def _check_route(n_experts, k, scoring, choice_bias, n_groups, kept_groups, group_score, scale):
+    """The refusals of d2dmoe_route_topk."""
+    if scoring not in SCORING or group_score not in GROUP_SCORE:
+        raise D2DMoEError(f'route_topk: scoring is one of {sorted(SCORING)}, group_score one of {sorted(GROUP_SCORE)}')
+    if n_groups < 1 or n_experts % n_groups or not 1 <= kept_groups <= n_groups or not 1 <= k <= kept_groups * (n_experts // n_groups):
+        raise D2DMoEError(f'route_topk: k = {k} of {n_experts} experts, {kept_groups} of {n_groups} groups kept')
+    if choice_bias is not None and choice_bias.shape != (n_experts,):
+        raise D2DMoEError(f'route_topk: choice_bias has shape {tuple(choice_bias.shape)}, expected ({n_experts},)')
+    if not abs(scale) < float('inf'):
+        raise D2DMoEError(f'route_topk: scale is finite, got {scale}')
+
+
 def route_topk_torch(logits, k, scoring='softmax', choice_bias=None, n_groups=1, kept_groups=1, group_score='top2',
                      renormalise=True, scale=1.0):
     """functional.route_topk composed in PyTorch, for tensors off the GPU: (routing, indices, weights), differentiable in the
     logits.  The choice goes by float64 scores, as in the kernel, the weights are float32 (float64 for float64 logits)."""
     n_experts = logits.size(-1)
+    _check_route(n_experts, k, scoring, choice_bias, n_groups, kept_groups, group_score, scale)
     z = logits.to(torch.promote_types(logits.dtype, torch.float32))
     with torch.no_grad():
         by = z.double()

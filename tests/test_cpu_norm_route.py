@@ -379,6 +379,21 @@ def test_layer_refuses_a_scale_that_routes_nothing(mode):
     assert ((moe.gate(x) > 0).sum(-1) == 3).all()
 
 
+def test_composed_route_refuses_what_the_kernel_call_refuses():
+    """The same settings of a gate must not answer on the CPU and raise on the GPU (or answer otherwise: any group_score but 'top2'
+    went as 'max', k beyond the kept groups left places over)."""
+    from d2dmoe_amd import D2DMoEError
+    from d2dmoe_amd.layer import route_topk_torch
+    z = torch.randn(2, 3, 8)
+    for kw in (dict(k=0), dict(k=9), dict(k=2, scoring='tanh'), dict(k=2, group_score='mean'), dict(k=2, n_groups=3), dict(k=2, n_groups=0),
+               dict(k=2, n_groups=4, kept_groups=0), dict(k=2, n_groups=4, kept_groups=5), dict(k=3, n_groups=4, kept_groups=1),
+               dict(k=2, kept_groups=2), dict(k=2, choice_bias=torch.zeros(1)), dict(k=2, choice_bias=torch.zeros(3, 8)),
+               dict(k=2, scale=math.inf), dict(k=2, scale=math.nan)):
+        with pytest.raises(D2DMoEError):
+            route_topk_torch(z, **kw)
+    assert route_topk_torch(z, 2, n_groups=4, kept_groups=1)[1].shape == (2, 3, 2)
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 
