@@ -98,7 +98,7 @@ def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bi
     lead = logits.shape[:-1]
     z = logits.reshape(-1, logits.size(-1)).contiguous()
     if choice_bias is not None:
-        choice_bias = choice_bias.detach()
+        choice_bias = choice_bias.detach().contiguous()
     args = (k, scoring, n_groups, kept_groups, group_score, renormalise, scale, want_counts)
     if _wanted(logits):
         routing, indices, weights, counts = _RouteTopk.apply(z, choice_bias, *args)

@@ -394,6 +394,18 @@ def test_composed_route_refuses_what_the_kernel_call_refuses():
     assert route_topk_torch(z, 2, n_groups=4, kept_groups=1)[1].shape == (2, 3, 2)
 
 
+def test_differentiable_route_copies_a_strided_bias(monkeypatch):
+    """As it does strided logits: a column of a table of biases is a bias."""
+    from d2dmoe_amd import functional, ops
+    got = []
+    monkeypatch.setattr(ops, 'route_topk', lambda z, k, scoring, bias, *args: (got.append((z, bias)), z, z[:, :k], z[:, :k], None)[1:])
+    table = torch.randn(8, 3)
+    z = torch.randn(8, 4).t()
+    functional.route_topk(z, 2, 'sigmoid', table[:, 1])
+    assert got[0][0].is_contiguous() and torch.equal(got[0][0], z)
+    assert got[0][1].is_contiguous() and torch.equal(got[0][1], table[:, 1])
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 
