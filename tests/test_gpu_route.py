@@ -132,6 +132,44 @@ def test_many_places(e, groups, k, t):
                 _check(z, k, scoring, bias, kw, t, got)
 
 
+@pytest.mark.parametrize('t', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('e,groups,kept,k', [(65, 1, 1, 65), (66, 33, 33, 66), (130, 2, 2, 65), (130, 2, 1, 65), (140, 70, 40, 66),
+                                             (256, 8, 4, 100), (513, 1, 1, 128), (1000, 10, 4, 333), (1024, 32, 16, 200),
+                                             (1024, 1024, 500, 70), (1024, 1, 1, 1024)])
+def test_more_places_than_a_wave_has_lanes(e, groups, kept, k, t):
+    """k > 64 runs on a kernel of its own: scores, biases, groups, masked and NaN rows, and the gradient of what it chose."""
+    n = 23 if k <= 66 else 8                                   # (the oracle's gradient takes k^2 steps a row)
+    for scoring in ('softmax', 'sigmoid'):
+        for score in ('top2', 'max'):
+            for biased in (True, False):
+                print('far', e, groups, kept, k, t, scoring, score, biased, flush=True)
+                z = _logits(n, e, t, seed=e + k, ties=score == 'max', masks=True)
+                bias = torch.randn(e, generator=torch.Generator().manual_seed(k)) * (0.1 if scoring == 'sigmoid' else 0.5 / e) if biased else None
+                if biased:
+                    bias[1] = -math.inf
+                    bias[e // 2] = torch.finfo(torch.float32).min
+                how = dict(renormalise=biased, scale=2.5)
+                kw = dict(n_groups=groups, kept_groups=kept, group_score=score, **how)
+                got = _ops().route_topk(z.to(DEV), k, scoring, None if bias is None else bias.to(DEV), want_counts=True, **kw)
+                idx, tol = _check(z, k, scoring, bias, kw, t, got)
+                q = torch.randn(n, k, generator=torch.Generator().manual_seed(e))
+                grad = _ops().route_topk_backward(z.to(DEV), got[1], scoring, grad_weights=q.to(DEV), **how)
+                _check_grad(z, idx, q.double().numpy(), scoring, how['renormalise'], 2.5, t, grad, tol)
+
+
+def test_more_places_than_lanes_with_biases_of_any_size():
+    g = torch.Generator().manual_seed(4)
+    e, lowest = 160, torch.finfo(torch.float32).min
+    z, some = _logits(40, e, torch.float32, seed=e), torch.rand(160, generator=g)
+    for bias in (torch.full((e,), 1000.0), some * 1e30, some * 1e-30, torch.where(some < 0.7, lowest, 0.0),
+                 torch.where(some < 0.5, 1e5, -1e5), torch.where(some < 0.3, math.inf, 0.0), torch.full((e,), -math.inf),
+                 torch.where(some < 0.9, 0.0, math.nan)):
+        for scoring in ('softmax', 'sigmoid'):
+            for kw in ({}, dict(n_groups=4, kept_groups=2, group_score='top2'), dict(n_groups=4, kept_groups=2, group_score='max')):
+                got = _ops().route_topk(z.to(DEV), 70, scoring, bias.to(DEV), want_counts=True, **kw)
+                _check(z, 70, scoring, bias, kw, torch.float32, got)
+
+
 def test_bias_that_is_not_a_number_routes_nothing():
     z = _logits(9, 32, torch.float32, seed=1)
     bias = torch.zeros(32)
@@ -497,3 +535,37 @@ def test_together_as_a_block_uses_them():
         served, gating = moe(idx, return_gating_data=True)
     assert (served - plain[0]).abs().max() <= 1e-4 * plain[0].abs().max()
     assert all(((g[0] > 0).sum(-1) == 4).all() for g in gating.values())
+
+
+def test_the_layer_calls_the_routing_function_once(monkeypatch):
+    """On the GPU a gate by scores is functional.route_topk, once per layer and pass; a substitute in its place is what runs."""
+    from d2dmoe_amd import add_routers, gpt2
+    from d2dmoe_amd.layer import route_topk_torch
+    import d2dmoe_amd.layer as layer_module
+    torch.manual_seed(6)
+    base = gpt2.GPT(gpt2.GPTConfig(block_size=16, vocab_size=32, n_layer=2, n_head=2, n_embd=64))
+    moe, names = gpt2.replace_with_moes(base, num_experts=8)
+    gpt2.split_original_parameters(base, moe, names)
+    add_routers(moe, dict(width=16, depth=2, bias=False, activation='relu', output_activation='identity'))
+    moe = moe.to(DEV)
+    for name in names:
+        lay = gpt2.get_module_by_name(moe, name)
+        lay.forward_mode, lay.k, lay.experts.forward_mode = 'sigmoid_topk', 2, 'masked'
+    calls = []
+    real = layer_module.functional.route_topk
+
+    def counted(run):
+        def call(z, *a, want_counts=False):
+            calls.append(run)
+            return real(z, *a, want_counts=want_counts) if run == 'hip' else (*route_topk_torch(z, *a), None)
+        return call
+
+    idx = torch.randint(0, 32, (2, 16), device=DEV)
+    found = {}
+    for run in ('hip', 'torch'):
+        with monkeypatch.context() as m:
+            m.setattr(layer_module.functional, 'route_topk', counted(run))
+            with torch.no_grad():
+                found[run] = moe(idx)
+    assert calls == ['hip'] * len(names) + ['torch'] * len(names) and layer_module.functional.route_topk is real
+    assert (found['hip'] - found['torch']).abs().max() <= 1e-4 * found['torch'].abs().max()
