@@ -17,11 +17,22 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
+def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.reshape(-1, t.shape[-1]).contiguous()
+
+
 class _LayerNorm(torch.autograd.Function):
+    """Takes and returns tensors of the caller's shape: x and residual have one gradient, and autograd copies it for the second
+    of two leaves only if both get the same tensor (not each a view of it, as a reshape ahead of this would make them)."""
+
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps):
-        out, total, mean, rstd = ops.layer_norm(x, weight, bias, eps, residual, want_stats=True)
-        ctx.save_for_backward(x if total is None else total, weight, mean, rstd)
+        rows = _rows(x)
+        out, total, mean, rstd = ops.layer_norm(rows, weight, bias, eps, _rows(residual), want_stats=True)
+        for t in (out, total):
+            if t is not None:
+                t.resize_(x.shape)      # (not a view: views that a Function returns refuse to be changed in place)
+        ctx.save_for_backward(rows if total is None else total, weight, mean, rstd)
         ctx.bias_type = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
         return out, total
@@ -33,10 +44,11 @@ class _LayerNorm(torch.autograd.Function):
         want_x, want_residual, want_weight, want_bias = ctx.needs_input_grad[:4]
         if grad_out is None:      # only the residual stream was used
             return (grad_sum if want_x else None, grad_sum if want_residual else None, None, None, None)
-        grad, gw, gb = ops.layer_norm_backward(grad_out.contiguous(), h, weight, mean, rstd,
-                                               None if grad_sum is None else grad_sum.contiguous(),
+        grad, gw, gb = ops.layer_norm_backward(_rows(grad_out), _rows(h), weight, mean, rstd, _rows(grad_sum),
                                                want_grad=want_x or want_residual, want_weight=want_weight, want_bias=want_bias,
                                                param_dtype=ctx.bias_type)
+        if grad is not None:
+            grad = grad.view(grad_out.shape)
         return (grad if want_x else None, grad if want_residual else None, gw, gb, None)
 
 
@@ -79,14 +91,13 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     shape = x.shape
     if residual is not None and residual.shape != shape:
         raise ops.abi.D2DMoEError(f'layer_norm: residual has shape {tuple(residual.shape)}, x {tuple(shape)}')
-    x2 = x.reshape(-1, shape[-1]).contiguous()
-    r2 = None if residual is None else residual.reshape(-1, shape[-1]).contiguous()
     weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
     if _wanted(x, residual, weight, bias):
-        out, total = _LayerNorm.apply(x2, r2, weight, bias, eps)
+        out, total = _LayerNorm.apply(x, residual, weight, bias, eps)
     else:
-        out, total, _, _ = ops.layer_norm(x2, weight, bias, eps, r2)
-    return out.view(shape) if residual is None else (out.view(shape), total.view(shape))
+        out, total, _, _ = ops.layer_norm(_rows(x), weight, bias, eps, _rows(residual))
+        out, total = out.view(shape), None if total is None else total.view(shape)
+    return out if residual is None else (out, total)
 
 
 def route_topk(logits: torch.Tensor, k: int, scoring: str = 'softmax', choice_bias: Optional[torch.Tensor] = None,

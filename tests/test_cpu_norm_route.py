@@ -406,6 +406,57 @@ def test_differentiable_route_copies_a_strided_bias(monkeypatch):
     assert got[0][1].is_contiguous() and torch.equal(got[0][1], table[:, 1])
 
 
+@pytest.mark.parametrize('shape', [(4, 8), (2, 2, 8), (8,), (0, 3, 8)])
+@pytest.mark.parametrize('strided', [False, True])
+def test_gradients_of_x_and_residual_are_tensors_of_their_own(shape, strided, monkeypatch):
+    """Both are the same numbers, computed once.  As two views of one tensor they became the .grad of two leaves in the same
+    memory, and a second backward pass added itself to it twice.  (Kernel calls replaced by a stream of ones.)"""
+    from d2dmoe_amd import functional, ops
+
+    def forward(x, w, b, eps, r, want_stats=False):
+        assert x.dim() == 2 and x.is_contiguous() and (r is None or r.is_contiguous())
+        return x * 1.0, None if r is None else x + r, torch.zeros(x.size(0)), torch.ones(x.size(0))
+
+    def backward(g, h, w, mean, rstd, gs=None, want_grad=True, want_weight=True, want_bias=True, param_dtype=None):
+        assert g.shape == h.shape and g.is_contiguous() and (gs is None or gs.shape == h.shape and gs.is_contiguous())
+        return g.clone() if gs is None else g + gs, None, None
+
+    monkeypatch.setattr(ops, 'layer_norm', forward)
+    monkeypatch.setattr(ops, 'layer_norm_backward', backward)
+
+    def leaf():
+        t = torch.randn(shape)
+        return (t.transpose(0, -1).contiguous().transpose(0, -1) if strided else t).requires_grad_()
+
+    for use in ('both', 'out', 'sum'):
+        x, r = leaf(), leaf()
+        for i in range(1, 4):
+            out, h = functional.layer_norm(x, residual=r)
+            assert out.shape == h.shape == shape
+            loss = (out.sum() if use != 'sum' else 0) + (h.sum() if use != 'out' else 0)
+            loss.backward()
+            each = 2.0 * i if use == 'both' else float(i)
+            assert (x.grad == each).all() and (r.grad == each).all()
+        if x.numel():
+            assert x.grad.data_ptr() != r.grad.data_ptr()
+    # what comes back may be changed in place, and what the backward pass needs may not unseen
+    x, r = leaf(), leaf()
+    out, h = functional.layer_norm(x, residual=r)
+    out.mul_(2.0)
+    (out.sum() + h.sum()).backward()
+    assert (x.grad == 3.0).all() and (r.grad == 3.0).all()
+    out, h = functional.layer_norm(x, residual=r)
+    h.add_(1.0)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+    # one tensor in both places
+    x = leaf()
+    for i in range(1, 3):
+        out, h = functional.layer_norm(x, residual=x)
+        out.sum().backward()
+        assert (x.grad == 2.0 * i).all()
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 

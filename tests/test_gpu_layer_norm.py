@@ -399,3 +399,17 @@ def test_models_under_autocast(t):
         for k in a[1]:
             assert a[1][k].dtype == c[1][k].dtype and torch.isfinite(c[1][k]).all()
             assert (a[1][k] - c[1][k]).norm() <= bound * torch.maximum(a[1][k].norm(), a[3][k]), k
+
+
+def test_gradients_add_up_over_backward_passes():
+    """Leaves with leading dimensions, three passes: the same gradients three times (float32; two additions of a half step each)."""
+    from d2dmoe_amd import functional
+    x, r, w, b, go, gs = _inputs(12, 64, torch.float32, torch.float32, seed=11)
+    leaves = [v.view(3, 4, 64).to(DEV).requires_grad_() for v in (x, r)] + [v.to(DEV).requires_grad_() for v in (w, b)]
+    go, gs = go.view(3, 4, 64).to(DEV), gs.view(3, 4, 64).to(DEV)
+    once = torch.autograd.grad(functional.layer_norm(leaves[0], leaves[2], leaves[3], 1e-5, leaves[1]), leaves, (go, gs))
+    for _ in range(3):
+        torch.autograd.backward(functional.layer_norm(leaves[0], leaves[2], leaves[3], 1e-5, leaves[1]), (go, gs))
+    assert len({v.grad.data_ptr() for v in leaves}) == 4
+    for v, g in zip(leaves, once):
+        assert ((v.grad - 3 * g).abs() <= 8 * U * g.abs()).all()
