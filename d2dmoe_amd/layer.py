@@ -218,7 +218,7 @@ class MoeficationMoE(MoELayer):
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
         saved = state_dict.get(prefix + 'balance_bias')
         if saved is not None and self.balance_bias is None:      # saved with one: the layer gets one
-            self.balance_bias = torch.empty_like(saved, device=next(self.parameters()).device)
+            self.balance_bias = torch.empty(self.num_experts, dtype=saved.dtype, device=next(self.parameters()).device)
         super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
     # ------------------------------------------------------------------------------ gating

@@ -457,6 +457,19 @@ def test_gradients_of_x_and_residual_are_tensors_of_their_own(shape, strided, mo
         assert (x.grad == 2.0 * i).all()
 
 
+def test_a_saved_bias_of_another_number_of_experts_does_not_load():
+    """A layer without a balance bias takes a saved one, of its own number of experts only."""
+    from d2dmoe_amd import MoeficationMoE
+    moe, other = (MoeficationMoE('m', 16, 8, True, 4, torch.nn.ReLU) for _ in range(2))
+    state = moe.state_dict()
+    state['balance_bias'] = torch.zeros(7)
+    with pytest.raises(RuntimeError, match='balance_bias'):
+        other.load_state_dict(state)
+    state['balance_bias'] = torch.arange(8.0)
+    other.load_state_dict(state)
+    assert torch.equal(other.balance_bias, torch.arange(8.0))
+
+
 class _Standin:
     """A tensor as far as the device check goes; -1: on the CPU."""
 
