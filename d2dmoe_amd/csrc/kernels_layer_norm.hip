@@ -515,7 +515,9 @@ inline int slab_count(int64_t N) { return (int)(N < 64 ? 1 : (cdiv64(N, 64) < 25
 // enough, then a workgroup of 256, of 1024.  Forward four; backward three, whose sums and the row ahead make 240 of the 256
 // registers that two waves per SIMD leave each thread.  There 1024 threads have 128, room for one vector (8192 x 8192 bf16:
 // 110 us), and wider rows take 512 threads: 8192 x 12288 bf16 160 us (5.0 TB/s), with 1024 threads of two vectors, which spilled,
-// 471; four vectors spill up to 24 registers and wait for their row (8192 x 16384: 250 us, 4.3 TB/s).
+// 471; four vectors spill up to 21 registers and wait for their row (8192 x 16384: 250 us, 4.3 TB/s).  Forward, 1024 threads have
+// no room for four vectors either (up to 23 registers spilled without a residual, 61 with one): 8192 x 32768 bf16 runs at 4.4 TB/s
+// and 3.6 with a residual; three vectors spill with one (up to 17) and reach 5.0 TB/s all the same, two 5.3.
 struct RowPlan { int tpr, ch; };
 template <typename T> RowPlan row_plan(int D, bool forward) {
   constexpr int V = kVec<T>;

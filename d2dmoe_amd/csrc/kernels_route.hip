@@ -54,10 +54,13 @@ __device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
 // other score of a pair shares; sigmoid: 4.2 u) and its sum with a bias by u |c| more.  Where two choices whose order matters
 // lie within 2^-19 + 2^-22 |c| of each other (sums of two scores: twice that) -- places next to one another in the list, the
 // last place and the first one left out, a group that stays and one that goes -- the wave repeats its choice on float64
-// scores; a row or two in a thousand do.  Their waves finish last: 16384 x 256 takes 16.8 us with a bias, of which 4.5 us are that
-// tail, and 30 us with one (all zeros, 16-bit logits) that leaves every wave in doubt.
+// scores; and so does a group whose two large biases cancel.  A row or two in a thousand do for logits of spread 1.5 and for
+// sigmoid scores.  Their waves finish last: 16384 x 256 takes 16.8 us with a bias, of which 4.5 us are that tail, and 30 us with
+// one (all zeros, 16-bit logits) that leaves every wave in doubt.  The doubt does not follow a score's size, so the softmax of
+// many small logits, whose scores lie closer together, has about half its waves in it: logits of spread 0.1 with a zero bias take
+// 16.4, 29.8 and 49.8 us at 16384 x 128, 256 and 512 float32, logits of spread 1.5 12.1, 17.6 and 25.6 us.
 //
-// Bound by vector instructions, not by memory: 388 per wave of four tokens at 128 experts and 8 places in bf16, 776 per wave
+// Bound by vector instructions, not by memory: 388 per wave of four tokens at 128 experts and 8 places in bf16, 789 per wave
 // of two at 256 in float32 with groups and a bias.  50432 x 128 bf16: 11 us (29 MB: 5.6 us at this card's copy rate);
 // 16384 x 256 float32 in groups: 20 us (35 MB: 6.7 us), 131072 x 256: 86 us.  Before: one wave per token with float64
 // throughout, 396 us for the first and 206 us for the second.

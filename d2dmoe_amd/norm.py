@@ -2,9 +2,13 @@
 ``forward_mode``.
 
 ``'torch'`` (the default) is ``F.layer_norm``, and the residual addition ahead of a block's second norm a tensor addition of
-its own.  ``'hip'`` runs the layer-norm kernels, forward and backward, with that addition inside (``add_norm``).  The two
-modes round alike at the tensors they store (the residual stream, the norm's output) and differ in the last bit of the
-latter at most."""
+its own.  ``'hip'`` runs the layer-norm kernels, forward and backward, with that addition inside (``add_norm``).  Both modes
+store the same tensors in the same element types.  The residual stream has the same bits; the norm's output differs by the
+float32 roundings of the row's sums, taken in another order: a few 2^-24 of |n w| + |b|, so 16-bit values now and then by
+a step, float32 ones in their last bits, and by more of their own size where n w + b comes near zero.
+
+Hooks on a norm that ``add_norm`` calls see what the mode passes: (x) and the output in ``'torch'`` mode, (x, residual) with
+the sum not yet taken, and the pair (output, sum), in ``'hip'`` mode."""
 from __future__ import annotations
 
 import torch
